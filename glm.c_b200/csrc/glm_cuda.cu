@@ -17,6 +17,7 @@
 
 #include "glm_cuda.h"
 #include "glm_internal.h"
+#include "serve_common.h"
 
 namespace glmq {
 
@@ -419,6 +420,11 @@ int moe_enqueue(int layer, float* x_dev, int n_tokens, int32_t* idx_dev, float* 
 }  // namespace
 
 void glmq::set_last_error(const char* msg) { g_err = msg ? msg : ""; }
+
+void glmq::count_launches(int n) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    g.launches += n;
+}
 
 namespace {
 

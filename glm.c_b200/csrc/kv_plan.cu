@@ -1,0 +1,215 @@
+// Block tables, slot maps and positions of a step's new tokens, from request
+// lengths, on the device: glm_cuda_kv_plan_async. glm.c keeps one contiguous
+// cache and a position counter for its single sequence (RunState, model.h:126;
+// the loop of infer.c:2190-2228); this is what takes their place when many
+// requests share a pool of pages.
+//
+// Request i has c_i positions in pages it already holds and gets n_i new
+// tokens. With pages of P positions it needs
+//   need_i = ceil((c_i + n_i) / P) - ceil(c_i / P)
+// pages more, which it takes from the free list in request order: from
+// first_i = sum_{j<i} need_j. Token j of the step belongs to the request with
+// start_i <= j < start_i + n_i, start_i = sum_{j<i} n_j, and goes to position
+// p = c_i + j - start_i, slot page(i, p / P) * P + p % P.
+//
+// One launch. Every CTA forms both running sums over all requests itself (at
+// most 16384 of them: 8 bytes read and two additions a request, no exchange
+// between CTAs and nothing to wait for), then takes its share of the tokens
+// and of the fresh pages, finding a token's request by bisection in shared
+// memory. Tokens are shared out evenly however unevenly the requests hold
+// them.
+#include <climits>
+#include <cstdint>
+
+#include "glm_internal.h"
+#include "q80_common.cuh"
+#include "serve_common.h"
+
+namespace glmq {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxReq = 16384;
+constexpr int kPlanTokens = 4;  // consecutive tokens a thread writes together
+
+struct PlanArgs {
+    const int32_t *cached, *fresh;
+    int n_req, page, n_free, stride, max_tokens;
+    const int32_t* free_pages;
+    int32_t* table;
+    int64_t* slots;
+    int32_t *positions, *token_req, *token_start, *summary;
+};
+
+struct Sums {
+    long long tokens, pages;
+};
+
+__device__ __forceinline__ Sums warp_scan(Sums v, int lane) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, v.tokens, off), p = __shfl_up_sync(0xffffffffu, v.pages, off);
+        if (lane >= off) {
+            v.tokens += t;
+            v.pages += p;
+        }
+    }
+    return v;
+}
+
+__device__ __forceinline__ int saturate(long long v) { return v > INT_MAX ? INT_MAX : (int)v; }
+
+__device__ __forceinline__ long long pages_of(long long n, int page) { return (n + page - 1) / page; }
+
+// Last i in [0, n) with s[i] <= v, for s[0] = 0 <= v: the entry that holds v.
+__device__ __forceinline__ int holder(const int* s, int n, int v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s[mid] <= v)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
+    extern __shared__ int plan_sm[];
+    int* start = plan_sm;                 // [n_req + 1] first token of each request
+    int* first = plan_sm + a.n_req + 1;   // [n_req + 1] first fresh page of each request
+    __shared__ Sums warp_tot[kPlanThreads / 32];
+    __shared__ int status_bits;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) status_bits = 0;
+    pdl_enter();
+
+    // running sums: a thread takes `per` consecutive requests
+    const int per = (a.n_req + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
+    Sums mine{0, 0};
+    int bits = 0;
+    for (int r = r0; r < r1; ++r) {
+        const int c = a.cached[r], n = a.fresh[r];
+        if (c < 0 || n < 0) bits |= 8;
+        const long long cc = max(c, 0), nn = max(n, 0);
+        if (pages_of(cc + nn, a.page) > a.stride) bits |= 2;
+        mine.tokens += nn;
+        mine.pages += pages_of(cc + nn, a.page) - pages_of(cc, a.page);
+    }
+    Sums run = warp_scan(mine, lane);
+    if (lane == 31) warp_tot[warp] = run;
+    __syncthreads();
+    if (warp == 0) {
+        const Sums w = warp_scan(warp_tot[lane], lane);
+        warp_tot[lane] = w;
+    }
+    if (bits) atomicOr(&status_bits, bits);
+    __syncthreads();
+    Sums at{run.tokens - mine.tokens, run.pages - mine.pages};
+    if (warp > 0) {
+        at.tokens += warp_tot[warp - 1].tokens;
+        at.pages += warp_tot[warp - 1].pages;
+    }
+    for (int r = r0; r < r1; ++r) {
+        start[r] = saturate(at.tokens);
+        first[r] = saturate(at.pages);
+        const long long cc = max(a.cached[r], 0), nn = max(a.fresh[r], 0);
+        at.tokens += nn;
+        at.pages += pages_of(cc + nn, a.page) - pages_of(cc, a.page);
+    }
+    const Sums total = warp_tot[kPlanThreads / 32 - 1];
+    if (tid == 0) {
+        start[a.n_req] = saturate(total.tokens);
+        first[a.n_req] = saturate(total.pages);
+    }
+    __syncthreads();
+
+    const int n_tokens = start[a.n_req], n_fresh = first[a.n_req];
+    const int gtid = blockIdx.x * kPlanThreads + tid, gthreads = gridDim.x * kPlanThreads;
+    if (gtid == 0) {
+        a.summary[0] = n_tokens;
+        a.summary[1] = n_fresh;
+        a.summary[2] = status_bits | (n_fresh > a.n_free ? 1 : 0) | (n_tokens > a.max_tokens ? 4 : 0);
+        a.summary[3] = 0;
+    }
+    for (int i = gtid; i <= a.n_req; i += gthreads) a.token_start[i] = start[i];
+
+    // fresh pages into their requests' tables; past the free list: -1
+    for (long long k = gtid; k < n_fresh; k += gthreads) {
+        const int i = holder(first, a.n_req, (int)k);
+        const long long col = pages_of(max(a.cached[i], 0), a.page) + (k - first[i]);
+        if (col < a.stride) a.table[(size_t)i * a.stride + col] = k < a.n_free ? a.free_pages[k] : -1;
+    }
+
+    // tokens, kPlanTokens consecutive ones to a thread
+    for (long long j0 = (long long)gtid * kPlanTokens; j0 < a.max_tokens; j0 += (long long)gthreads * kPlanTokens) {
+        int i = j0 < n_tokens ? holder(start, a.n_req, (int)j0) : 0;
+        int64_t slot[kPlanTokens];
+        int pos[kPlanTokens], req[kPlanTokens];
+#pragma unroll
+        for (int u = 0; u < kPlanTokens; ++u) {
+            const int j = (int)(j0 + u);
+            slot[u] = -1;
+            pos[u] = req[u] = -1;
+            if (j < n_tokens && j < a.max_tokens) {
+                while (start[i + 1] <= j) ++i;  // requests without tokens are stepped over
+                const long long c = max(a.cached[i], 0), p = c + (j - start[i]);
+                const long long col = p / a.page, held = pages_of(c, a.page);
+                int id = -1;
+                if (col < held) {
+                    if (col < a.stride) id = a.table[(size_t)i * a.stride + col];
+                } else if (col < a.stride) {
+                    const long long k = first[i] + (col - held);
+                    if (k < a.n_free) id = a.free_pages[k];
+                }
+                pos[u] = saturate(p);
+                req[u] = i;
+                if (id >= 0) slot[u] = (int64_t)id * a.page + (p - col * a.page);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kPlanTokens; ++u)
+            if (j0 + u < a.max_tokens) {
+                a.slots[j0 + u] = slot[u];
+                a.positions[j0 + u] = pos[u];
+                a.token_req[j0 + u] = req[u];
+            }
+    }
+}
+
+}  // namespace
+}  // namespace glmq
+
+extern "C" int glm_cuda_kv_plan_async(const int32_t* cached_len_dev, const int32_t* new_len_dev, int n_req,
+                                      int page_size, const int32_t* free_pages_dev, int n_free,
+                                      int32_t* block_table_dev, int table_stride, int max_tokens,
+                                      int64_t* slot_map_dev, int32_t* positions_dev, int32_t* token_req_dev,
+                                      int32_t* token_start_dev, int32_t* summary_dev, void* stream) {
+    using namespace glmq;
+    const char* fn = "glm_cuda_kv_plan_async";
+    if (!cached_len_dev || !new_len_dev || !block_table_dev || !token_start_dev || !summary_dev)
+        return op_fail(GLM_CUDA_ERR_ARG, fn, "a required pointer is NULL");
+    if (n_req < 1 || n_req > kPlanMaxReq) return op_fail(GLM_CUDA_ERR_ARG, fn, "n_req=%d (need 1..%d)", n_req, kPlanMaxReq);
+    if (page_size < 1 || table_stride < 1) return op_fail(GLM_CUDA_ERR_ARG, fn, "page_size=%d table_stride=%d", page_size, table_stride);
+    if (n_free < 0 || (n_free > 0 && !free_pages_dev)) return op_fail(GLM_CUDA_ERR_ARG, fn, "n_free=%d without a list", n_free);
+    if (max_tokens < 0 || (max_tokens > 0 && (!slot_map_dev || !positions_dev || !token_req_dev)))
+        return op_fail(GLM_CUDA_ERR_ARG, fn, "max_tokens=%d without its outputs", max_tokens);
+    int sms = 0;
+    if (cudaError_t e = current_sms(&sms)) return launch_failed(fn, e);
+    const size_t smem = 2 * sizeof(int) * ((size_t)n_req + 1);
+    const long long items = (long long)kPlanThreads * kPlanTokens;
+    long long grid = (max_tokens + items - 1) / items;
+    grid = grid < 1 ? 1 : grid > sms ? sms : grid;
+    try {
+        cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kv_plan_kernel), (int)smem);
+        PlanArgs a{cached_len_dev, new_len_dev, n_req, page_size, n_free, table_stride, max_tokens, free_pages_dev,
+                   block_table_dev, slot_map_dev, positions_dev, token_req_dev, token_start_dev, summary_dev};
+        if (!e) e = launch_pdl(kv_plan_kernel, (unsigned)grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
+        if (e) return launch_failed(fn, e);
+        count_launches(1);
+    } catch (...) {
+        return op_fail(GLM_CUDA_ERR_NOMEM, fn, "host allocation failed");
+    }
+    return 0;
+}

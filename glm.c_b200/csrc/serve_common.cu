@@ -1,0 +1,59 @@
+// Host-side helpers of the entry points that serve many requests (serve_common.h).
+#include <cstdarg>
+#include <cstdio>
+#include <mutex>
+
+#include "glm_internal.h"
+#include "kv4.cuh"
+#include "serve_common.h"
+
+namespace glmq {
+
+int op_fail(int code, const char* fn, const char* fmt, ...) {
+    char what[384], msg[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(what, sizeof what, fmt, ap);
+    va_end(ap);
+    snprintf(msg, sizeof msg, "%s: %s", fn, what);
+    set_last_error(msg);
+    fprintf(stderr, "[glm-cuda] %s\n", msg);
+    return code;
+}
+
+int launch_failed(const char* fn, cudaError_t e) {
+    cudaGetLastError();  // a refused launch leaves nothing behind for the next call
+    return op_fail(GLM_CUDA_ERR_CUDA, fn, "launch failed: %s", cudaGetErrorString(e));
+}
+
+cudaError_t current_sms(int* sms) {
+    constexpr int kMaxDevices = 64;
+    static std::mutex mu;
+    static int known[kMaxDevices];
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lk(mu);
+    if (known[dev] == 0)
+        if (cudaError_t e = cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev)) return e;
+    *sms = known[dev];
+    return cudaSuccess;
+}
+
+int check_kv4_cache(const char* fn, const GlmCudaKv4Cache* c) {
+    if (!c || !c->pages || c->n_pages <= 0) return op_fail(GLM_CUDA_ERR_ARG, fn, "no cache pages");
+    if (!kv4_shape_ok(c->kv_lora_rank, c->rope_dim, c->page_size))
+        return op_fail(GLM_CUDA_ERR_ARG, fn,
+                       "unsupported cache kv_lora_rank=%d rope_dim=%d page_size=%d (need 128, 256, 384 or 512; 64 or "
+                       "128; 16, 32, 64, 128 or 256)",
+                       c->kv_lora_rank, c->rope_dim, c->page_size);
+    if (!aligned(c->pages, 16)) return op_fail(GLM_CUDA_ERR_ARG, fn, "cache pages must be 16-byte aligned");
+    return 0;
+}
+
+}  // namespace glmq
+
+extern "C" size_t glm_cuda_kv4_page_bytes(int kv_lora_rank, int rope_dim, int page_size) {
+    if (!glmq::kv4_shape_ok(kv_lora_rank, rope_dim, page_size)) return 0;
+    return glmq::Kv4Shape{kv_lora_rank, rope_dim, page_size}.page_bytes();
+}

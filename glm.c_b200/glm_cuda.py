@@ -40,6 +40,7 @@ def declared_functions(header: str = HEADER) -> list[str]:
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
 
 
 def _signatures(L: ctypes.CDLL) -> None:
@@ -103,6 +104,21 @@ def _signatures(L: ctypes.CDLL) -> None:
         getattr(L, name).restype = _I
 
 
+    L.glm_cuda_kv4_page_bytes.argtypes = [_I] * 3
+    L.glm_cuda_kv4_page_bytes.restype = ctypes.c_size_t
+    L.glm_cuda_kv_plan_async.argtypes = [_P, _P, _I, _I, _P, _I, _P, _I, _I] + [_P] * 6
+    L.glm_cuda_kv4_store_async.argtypes = [_P, _P, _L, _P, _L, _I, _P, _I, _P]
+    L.glm_cuda_kv4_load_async.argtypes = [_P, _P, _I, _P, _L, _P, _L, _I, _P]
+    L.glm_cuda_mla4_workspace_bytes.argtypes = [_I] * 3
+    L.glm_cuda_mla4_workspace_bytes.restype = ctypes.c_size_t
+    L.glm_cuda_mla4_attention_async.argtypes = [_P, _P, _I, _L, _L, _P, _I, _I, _P, _P, _I, _I, ctypes.c_float, _P, _L,
+                                                _L, _P, _P, ctypes.c_size_t, _P]
+    L.glm_cuda_logprobs_async.argtypes = [_P, _I, _L, _I, _I, _P, _P, _P, _I, _P, _P, _P]
+    for name in ("glm_cuda_kv_plan_async", "glm_cuda_kv4_store_async", "glm_cuda_kv4_load_async",
+                 "glm_cuda_mla4_attention_async", "glm_cuda_logprobs_async"):
+        getattr(L, name).restype = _I
+
+
 _lib = None
 
 
@@ -127,6 +143,41 @@ def _ptr(a) -> int | None:
     if isinstance(a, np.ndarray):
         return a.ctypes.data
     return a.data_ptr()  # torch tensor
+
+
+class Kv4Cache(ctypes.Structure):
+    """GlmCudaKv4Cache; `tensor` keeps the pool alive."""
+
+    _fields_ = [("pages", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("kv_lora_rank", ctypes.c_int32),
+                ("rope_dim", ctypes.c_int32), ("page_size", ctypes.c_int32)]
+
+
+_TYPES: dict = {}  # torch dtype -> GLM_CUDA_F32 / _BF16 / _F16
+
+
+def _type(t) -> int:
+    if not _TYPES:
+        import torch
+
+        _TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    try:
+        return _TYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{t.dtype}: float32, bfloat16 or float16 is needed") from None
+
+
+def _int_tensor(name: str, t, dtype: str, shape=None) -> None:
+    """Refuse what the C entry point could not tell: a tensor of another type, off the GPU, with gaps or too small."""
+    if str(t.dtype) != dtype or not t.is_cuda or not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"{name}: a contiguous CUDA tensor of {dtype}{'' if shape is None else f' {shape}'} is needed, "
+                         f"not {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _rows(name: str, t, shape) -> None:
+    """A CUDA tensor of `shape` whose last dimension has no gaps."""
+    if not t.is_cuda or tuple(t.shape) != shape or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name}: a CUDA tensor {shape} with a dense last dimension is needed, not {tuple(t.shape)} "
+                         f"strides {t.stride()} on {t.device}")
 
 
 class GlmCuda:
@@ -336,6 +387,115 @@ class GlmCuda:
         self._check("glm_cuda_matvec_q80_async",
                     self.L.glm_cuda_matvec_q80_async(_ptr(q_dev), _ptr(s_dev), _ptr(x_dev), _ptr(y_dev), rows,
                                                      cols, gs, stream))
+
+    # ---- many requests over the paged 4-bit latent cache (torch tensors on the current device; no init needed)
+    def kv4_page_bytes(self, kv_lora: int, rope: int, page_size: int) -> int:
+        return int(self.L.glm_cuda_kv4_page_bytes(kv_lora, rope, page_size))
+
+    def kv4_cache(self, pages, n_pages: int, kv_lora: int, rope: int, page_size: int) -> Kv4Cache:
+        """The cache description of a pool of n_pages pages in the uint8 tensor `pages`."""
+        need = self.kv4_page_bytes(kv_lora, rope, page_size) * n_pages
+        if need == 0 or not pages.is_cuda or not pages.is_contiguous() or pages.numel() * pages.element_size() < need:
+            raise ValueError(f"kv4_cache: {n_pages} pages of kv_lora {kv_lora}, rope {rope}, page_size {page_size} need "
+                             f"{need} contiguous bytes on the GPU")
+        c = Kv4Cache(pages.data_ptr(), n_pages, kv_lora, rope, page_size)
+        c.tensor = pages
+        c.ref = ctypes.addressof(c)
+        return c
+
+    def kv_plan_async(self, cached_len, new_len, page_size: int, free_pages, block_table, max_tokens: int, slot_map,
+                      positions, token_req, token_start, summary, stream=None) -> None:
+        """Block tables and slots of a step's new tokens (block_table [n_req, stride] is updated in place)."""
+        n_req = cached_len.shape[0]
+        _int_tensor("cached_len", cached_len, "torch.int32")
+        _int_tensor("new_len", new_len, "torch.int32", (n_req,))
+        _int_tensor("free_pages", free_pages, "torch.int32")
+        _int_tensor("block_table", block_table, "torch.int32", (n_req, block_table.shape[-1]))
+        _int_tensor("slot_map", slot_map, "torch.int64", (max_tokens,))
+        _int_tensor("positions", positions, "torch.int32", (max_tokens,))
+        _int_tensor("token_req", token_req, "torch.int32", (max_tokens,))
+        _int_tensor("token_start", token_start, "torch.int32", (n_req + 1,))
+        _int_tensor("summary", summary, "torch.int32", (4,))
+        rc = self.L.glm_cuda_kv_plan_async(cached_len.data_ptr(), new_len.data_ptr(), n_req, page_size,
+                                           free_pages.data_ptr(), free_pages.numel(), block_table.data_ptr(),
+                                           block_table.shape[1], max_tokens, slot_map.data_ptr(), positions.data_ptr(),
+                                           token_req.data_ptr(), token_start.data_ptr(), summary.data_ptr(), stream)
+        if rc:
+            self._check("glm_cuda_kv_plan_async", rc)
+
+    def kv4_store_async(self, cache: Kv4Cache, latent, rope, slots, stream=None) -> None:
+        """Rows latent [n, kv_lora] and rope [n, rope] quantised into their slots."""
+        n = slots.numel()
+        _int_tensor("slots", slots, "torch.int64")
+        _rows("latent", latent, (n, cache.kv_lora_rank))
+        _rows("rope", rope, (n, cache.rope_dim))
+        if latent.dtype != rope.dtype:
+            raise ValueError("latent and rope differ in type")
+        rc = self.L.glm_cuda_kv4_store_async(cache.ref, latent.data_ptr(), latent.stride(0), rope.data_ptr(),
+                                             rope.stride(0), _type(latent), slots.data_ptr(), n, stream)
+        if rc:
+            self._check("glm_cuda_kv4_store_async", rc)
+
+    def kv4_load_async(self, cache: Kv4Cache, slots, latent, rope, stream=None) -> None:
+        """The rows in `slots` into latent [n, kv_lora] and rope [n, rope]."""
+        n = slots.numel()
+        _int_tensor("slots", slots, "torch.int64")
+        _rows("latent", latent, (n, cache.kv_lora_rank))
+        _rows("rope", rope, (n, cache.rope_dim))
+        if latent.dtype != rope.dtype:
+            raise ValueError("latent and rope differ in type")
+        rc = self.L.glm_cuda_kv4_load_async(cache.ref, slots.data_ptr(), n, latent.data_ptr(), latent.stride(0),
+                                            rope.data_ptr(), rope.stride(0), _type(latent), stream)
+        if rc:
+            self._check("glm_cuda_kv4_load_async", rc)
+
+    def mla4_workspace_bytes(self, n_rows: int, n_heads: int, kv_lora: int) -> int:
+        return int(self.L.glm_cuda_mla4_workspace_bytes(n_rows, n_heads, kv_lora))
+
+    def mla4_attention_async(self, cache: Kv4Cache, q, block_table, row_req, row_pos, scale: float, out, lse, ws,
+                             stream=None) -> None:
+        """Attention of q [n, heads, kv_lora + rope] over the cache into out [n, heads, kv_lora] and lse [n, heads]."""
+        n, heads = q.shape[0], q.shape[1]
+        _rows("q", q, (n, heads, cache.kv_lora_rank + cache.rope_dim))
+        _rows("out", out, (n, heads, cache.kv_lora_rank))
+        if q.dtype != out.dtype:
+            raise ValueError("q and out differ in type")
+        _int_tensor("block_table", block_table, "torch.int32", tuple(block_table.shape[-2:]))
+        _int_tensor("row_req", row_req, "torch.int32", (n,))
+        _int_tensor("row_pos", row_pos, "torch.int32", (n,))
+        if lse is not None:
+            _int_tensor("lse", lse, "torch.float32", (n, heads))
+        if not ws.is_cuda or not ws.is_contiguous():
+            raise ValueError("ws: contiguous CUDA memory is needed")
+        rc = self.L.glm_cuda_mla4_attention_async(
+            cache.ref, q.data_ptr(), _type(q), q.stride(0), q.stride(1), block_table.data_ptr(), block_table.shape[1],
+            block_table.shape[0], row_req.data_ptr(), row_pos.data_ptr(), n, heads, scale, out.data_ptr(),
+            out.stride(0), out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size(), stream)
+        if rc:
+            self._check("glm_cuda_mla4_attention_async", rc)
+
+    def logprobs_async(self, logits, target=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None,
+                       stream=None) -> None:
+        """Rows of logits [n, vocab]: log probability of target [n], entropy [n], top_ids and top_logprobs [n, k]."""
+        n, vocab = logits.shape
+        _rows("logits", logits, (n, vocab))
+        k = 0
+        if (top_ids is None) != (top_logprobs is None):
+            raise ValueError("top_ids and top_logprobs go together")
+        if top_ids is not None:
+            k = top_ids.shape[-1]
+            _int_tensor("top_ids", top_ids, "torch.int32", (n, k))
+            _int_tensor("top_logprobs", top_logprobs, "torch.float32", (n, k))
+        if target is not None:
+            _int_tensor("target", target, "torch.int32", (n,))
+        for name, t in (("logprob", logprob), ("entropy", entropy)):
+            if t is not None:
+                _int_tensor(name, t, "torch.float32", (n,))
+        rc = self.L.glm_cuda_logprobs_async(logits.data_ptr(), _type(logits), logits.stride(0), n, vocab, _ptr(target),
+                                            _ptr(logprob), _ptr(entropy), k, _ptr(top_ids), _ptr(top_logprobs), stream)
+        if rc:
+            self._check("glm_cuda_logprobs_async", rc)
 
     def synchronize(self) -> None:
         self._check("glm_cuda_synchronize", self.L.glm_cuda_synchronize())

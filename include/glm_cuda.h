@@ -24,6 +24,7 @@
 #ifndef GLM_CUDA_H
 #define GLM_CUDA_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -373,6 +374,112 @@ int glm_cuda_set_model_prefill(int min_tokens);
 int glm_cuda_load_checkpoint(const char *path, int device, int cache_cap);
 
 void glm_cuda_free(void);
+
+/* ------------------------------------------------------------------------
+ * Many requests over a paged latent cache held in 4 bits. glm.c decodes one
+ * sequence over a contiguous fp32 cache (RunState, model.h:126-160); these
+ * calls are what a server that batches requests puts in its place:
+ *   glm_cuda_kv_plan_async        which slots a step's new tokens go to
+ *   glm_cuda_kv4_store_async      their latent rows into those slots, in 4 bits
+ *   glm_cuda_mla4_attention_async the tokens' attention over the cache
+ *   glm_cuda_logprobs_async       what the model said: log probabilities
+ *   glm_cuda_kv4_load_async       cached rows back as numbers
+ * They keep no state: no glm_cuda_init is needed, every pointer is device
+ * memory of the caller on the current device, nothing is allocated, and
+ * `stream` is a cudaStream_t (NULL: the legacy default stream). They return
+ * after enqueueing; the tensors must stay alive, and work on other streams
+ * ordered, until the stream has passed the call. Device contents that make
+ * no sense (a page or slot outside the pool, a request that is not there, a
+ * negative position) are never followed: see each call.
+ * ------------------------------------------------------------------------ */
+
+#define GLM_CUDA_F32 0
+#define GLM_CUDA_BF16 1
+#define GLM_CUDA_F16 2
+
+/* A pool of pages, each holding page_size positions of one layer's cache:
+ * the codes [page_size][(kv_lora_rank + rope_dim) / 2] (element 2b of a row
+ * in the low half of byte b, 2b + 1 in the high half, a code being v + 8 with
+ * v in [-7, 7]), then bf16 scales [kv_lora_rank / 128 + 1][page_size], one for
+ * every 128 latents and one for the rope part; an element is worth v times its
+ * scale. kv_lora_rank 128, 256, 384 or 512; rope_dim 64 or 128; page_size 16,
+ * 32, 64, 128 or 256; pages 16-byte aligned. */
+typedef struct GlmCudaKv4Cache {
+    void *pages;
+    int64_t n_pages;
+    int32_t kv_lora_rank, rope_dim, page_size;
+} GlmCudaKv4Cache;
+
+/* Bytes of one page (298 a position at 512 + 64); 0 for sizes not supported. */
+size_t glm_cuda_kv4_page_bytes(int kv_lora_rank, int rope_dim, int page_size);
+
+/* Slots of a step's new tokens. Request i has cached_len[i] positions in the
+ * pages that row i of block_table [n_req][table_stride] lists, and gets
+ * new_len[i] tokens. Pages that it needs on top are taken from free_pages
+ * [n_free] in request order and written into its row (the other entries stay
+ * as they are). The tokens, in request order, get
+ *   slot_map [max_tokens]   page * page_size + offset
+ *   positions [max_tokens]  their position in their request
+ *   token_req [max_tokens]  their request
+ * with -1 in all three past the last token, and token_start [n_req + 1] gets
+ * the first token of each request. summary[4]: tokens, pages taken, status
+ * bits (1: n_free was too small, 2: a request needs more than table_stride
+ * pages, 4: more tokens than max_tokens, 8: a negative length, taken as 0),
+ * 0. A token without a page gets slot -1 and a page that was not there is -1
+ * in the table. 1 <= n_req <= 16384; any page_size >= 1. free_pages may be
+ * NULL with n_free 0, the token arrays with max_tokens 0. */
+int glm_cuda_kv_plan_async(const int32_t *cached_len_dev, const int32_t *new_len_dev, int n_req, int page_size,
+                           const int32_t *free_pages_dev, int n_free, int32_t *block_table_dev, int table_stride,
+                           int max_tokens, int64_t *slot_map_dev, int32_t *positions_dev, int32_t *token_req_dev,
+                           int32_t *token_start_dev, int32_t *summary_dev, void *stream);
+
+/* Quantise rows (latent [n_rows][kv_lora_rank], rope [n_rows][rope_dim], of
+ * GLM_CUDA_F32, _BF16 or _F16, rows `stride` elements apart) into their slots:
+ * per group s = bf16(max |x| / 7), v = rint(x / s) clamped to [-7, 7]. A group
+ * with a NaN or an infinity gets the scale NaN. Rows whose slot is outside the
+ * pool (-1, say) are left out; two rows must not share a slot. */
+int glm_cuda_kv4_store_async(const GlmCudaKv4Cache *cache, const void *latent_dev, int64_t latent_stride,
+                             const void *rope_dev, int64_t rope_stride, int type, const int64_t *slots_dev, int n_rows,
+                             void *stream);
+
+/* The rows in the given slots as numbers (zeros for a slot outside the pool). */
+int glm_cuda_kv4_load_async(const GlmCudaKv4Cache *cache, const int64_t *slots_dev, int n_rows, void *latent_dev,
+                            int64_t latent_stride, void *rope_dev, int64_t rope_stride, int type, void *stream);
+
+/* MLA attention (infer.c:1020-1058 between the k_b and v_b products) of
+ * n_rows single tokens over the cache. Row r is the token at position
+ * row_pos[r] of request row_req[r] and sees the positions 0 .. row_pos[r] of
+ * its row of block_table [n_req][table_stride]. q [n_rows][n_heads][kv_lora_rank
+ * + rope_dim] holds the absorbed query (k_b_h q_nope, then the roped q_pe), out
+ * [n_rows][n_heads][kv_lora_rank] receives the context latents (v_b's input);
+ * both of type GLM_CUDA_BF16 or _F16, with row and head strides in elements.
+ * lse [n_rows][n_heads] (may be NULL) receives ln sum exp(scale * q . k). A
+ * position whose page lies outside the pool is not seen; a row that sees
+ * nothing (position -1, a request outside [0, n_req)) gives zeros and -inf.
+ * Sums and statistics are 32-bit; the probabilities are rounded to 8 bits
+ * of significance relative to each 64 positions' largest. 0 <= n_rows <=
+ * 16384, 1 <= n_heads <= 256. ws: glm_cuda_mla4_workspace_bytes() bytes,
+ * 16-byte aligned, not shared by calls that may overlap; its contents need
+ * no preparation. */
+size_t glm_cuda_mla4_workspace_bytes(int n_rows, int n_heads, int kv_lora_rank);
+int glm_cuda_mla4_attention_async(const GlmCudaKv4Cache *cache, const void *q_dev, int type, int64_t q_row_stride,
+                                  int64_t q_head_stride, const int32_t *block_table_dev, int table_stride, int n_req,
+                                  const int32_t *row_req_dev, const int32_t *row_pos_dev, int n_rows, int n_heads,
+                                  float scale, void *out_dev, int64_t out_row_stride, int64_t out_head_stride,
+                                  float *lse_dev, void *ws_dev, size_t ws_bytes, void *stream);
+
+/* Log probabilities of rows of logits [n_rows][vocab] (GLM_CUDA_F32, _BF16 or
+ * _F16, rows row_stride elements apart), read once. Per row:
+ *   logprob       that of target[row] (-inf for a target outside [0, vocab)); both may be NULL together
+ *   entropy       in nats (may be NULL)
+ *   top_ids, top_logprobs [n_rows][top_k]   the most likely tokens, equal ones by lowest id; 0 <= top_k <= 32
+ * A logit of -inf is a token that cannot be: it is never among the top
+ * tokens, whose places are then filled with -1 and -inf. A row of nothing but
+ * -inf has logprob -inf and entropy 0. A row with a NaN or +inf gives NaN
+ * (the top ids still go by value, NaN aside). */
+int glm_cuda_logprobs_async(const void *logits_dev, int type, int64_t row_stride, int n_rows, int vocab,
+                            const int32_t *target_dev, float *logprob_dev, float *entropy_dev, int top_k,
+                            int32_t *top_ids_dev, float *top_logprobs_dev, void *stream);
 
 #ifdef __cplusplus
 }

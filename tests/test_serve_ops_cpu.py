@@ -1,0 +1,104 @@
+"""Refusals of the entry points that serve many requests: arguments that no call takes return GLM_CUDA_ERR_ARG with
+a message before any CUDA call (the pointers here are never followed)."""
+import ctypes
+
+import pytest
+
+P = 1 << 20  # an address that no refused call may touch
+
+
+@pytest.fixture(scope="module")
+def gc(pkg):
+    pkg.build.build()
+    return pkg.glm_cuda
+
+
+@pytest.fixture(scope="module")
+def L(gc):
+    return gc.load()
+
+
+def cache(gc, pages=P, n_pages=4, kv=512, rope=64, page=64):
+    c = gc.Kv4Cache(pages, n_pages, kv, rope, page)
+    return c, ctypes.addressof(c)
+
+
+def refused(L, rc, word):
+    assert rc == -1, rc
+    assert word in L.glm_cuda_last_error().decode(), L.glm_cuda_last_error()
+
+
+def test_page_bytes(L):
+    assert L.glm_cuda_kv4_page_bytes(512, 64, 64) == 64 * 298
+    assert L.glm_cuda_kv4_page_bytes(128, 64, 16) == 16 * (96 + 4)
+    for bad in ((500, 64, 64), (640, 64, 64), (512, 32, 64), (512, 64, 48), (0, 64, 64), (512, 64, 0), (-128, 64, 64)):
+        assert L.glm_cuda_kv4_page_bytes(*bad) == 0
+
+
+def test_plan_refusals(L):
+    good = dict(cached=P, new=P, n=4, page=16, free=P, n_free=3, table=P, stride=8, m=5, slots=P, pos=P, req=P, start=P, summ=P)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return L.glm_cuda_kv_plan_async(a["cached"], a["new"], a["n"], a["page"], a["free"], a["n_free"], a["table"],
+                                        a["stride"], a["m"], a["slots"], a["pos"], a["req"], a["start"], a["summ"], None)
+
+    for kw, word in ((dict(cached=None), "NULL"), (dict(table=None), "NULL"), (dict(summ=None), "NULL"), (dict(n=0), "n_req"),
+                     (dict(n=16385), "n_req"), (dict(page=0), "page_size"), (dict(stride=0), "table_stride"),
+                     (dict(n_free=-1), "n_free"), (dict(free=None), "n_free"), (dict(m=-1), "max_tokens"),
+                     (dict(slots=None), "max_tokens")):
+        refused(L, call(**kw), word)
+
+
+def test_row_refusals(L, gc):
+    for call, name in ((lambda c, lat=P, ls=512, rp=P, rs=64, ty=0, sl=P, n=3: L.glm_cuda_kv4_store_async(c, lat, ls, rp, rs, ty, sl, n, None), "store"),
+                       (lambda c, lat=P, ls=512, rp=P, rs=64, ty=0, sl=P, n=3: L.glm_cuda_kv4_load_async(c, sl, n, lat, ls, rp, rs, ty, None), "load")):
+        _, ref = cache(gc)
+        keep = _
+        refused(L, call(None), "no cache")
+        for bad, word in ((dict(pages=None), "no cache"), (dict(n_pages=0), "no cache"), (dict(kv=100), "kv_lora"), (dict(rope=32), "rope"),
+                          (dict(page=24), "page_size"), (dict(pages=P + 8), "aligned")):
+            b, bref = cache(gc, **bad)
+            refused(L, call(bref), word)
+        for kw, word in ((dict(ty=3), "type"), (dict(n=-1), "n_rows"), (dict(lat=None), "NULL"), (dict(sl=None), "NULL"),
+                         (dict(ls=511), "strides"), (dict(rs=0), "strides"), (dict(lat=P + 2), "aligned"), (dict(sl=P + 4), "aligned")):
+            refused(L, call(ref, **kw), word)
+        assert name in L.glm_cuda_last_error().decode()
+        assert call(ref, n=0) == 0
+        del keep
+
+
+def test_attention_refusals(L, gc):
+    keep, ref = cache(gc)
+    need = L.glm_cuda_mla4_workspace_bytes(4, 20, 512)
+    good = dict(c=ref, q=P, ty=1, table=P, stride=8, n_req=4, req=P, pos=P, n=4, h=20, out=P, ws=P, wb=need)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return L.glm_cuda_mla4_attention_async(a["c"], a["q"], a["ty"], 20 * 576, 576, a["table"], a["stride"], a["n_req"],
+                                               a["req"], a["pos"], a["n"], a["h"], 0.1, a["out"], 20 * 512, 512, None,
+                                               a["ws"], a["wb"], None)
+
+    for kw, word in ((dict(c=None), "no cache"), (dict(ty=0), "type"), (dict(ty=7), "type"), (dict(n=-1), "n_rows"),
+                     (dict(n=16385), "n_rows"), (dict(h=0), "n_heads"), (dict(h=257), "n_heads"), (dict(n_req=0), "n_req"),
+                     (dict(stride=0), "table_stride"), (dict(q=None), "NULL"), (dict(table=None), "NULL"), (dict(out=None), "NULL"),
+                     (dict(ws=None), "NULL"), (dict(q=P + 1), "aligned"), (dict(ws=P + 4), "aligned"), (dict(wb=need - 1), "workspace")):
+        refused(L, call(**kw), word)
+    assert call(n=0) == 0
+    assert L.glm_cuda_mla4_workspace_bytes(0, 20, 512) == 0
+    del keep
+
+
+def test_logprob_refusals(L):
+    good = dict(x=P, ty=0, stride=100, n=3, v=100, t=P, lp=P, en=P, k=2, ids=P, tl=P)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return L.glm_cuda_logprobs_async(a["x"], a["ty"], a["stride"], a["n"], a["v"], a["t"], a["lp"], a["en"], a["k"],
+                                         a["ids"], a["tl"], None)
+
+    for kw, word in ((dict(ty=9), "type"), (dict(n=-1), "n_rows"), (dict(v=0), "vocab"), (dict(stride=99), "row_stride"),
+                     (dict(k=33), "top_k"), (dict(k=-1), "top_k"), (dict(x=None), "logits"), (dict(x=P + 2), "logits"),
+                     (dict(t=None), "target"), (dict(lp=None), "target"), (dict(ids=None), "top_k"), (dict(tl=None), "top_k")):
+        refused(L, call(**kw), word)
+    assert call(n=0) == 0

@@ -1,0 +1,585 @@
+"""The operators that serve many requests over the paged 4-bit latent cache, against plain implementations in
+64 bits: plan (block tables, slot maps), cache rows stored and loaded, MLA attention, log probabilities.
+
+Tolerances, from the number formats:
+* plan, codes, scales, ids: equal.
+* loaded rows: v * s in fp32 is exact (3 + 8 bits), then one rounding to the output's type.
+* attention: the probabilities carry 8 significant bits (2^-9 relative at most, 1.1e-3 rms) and the output one
+  rounding to bf16 (up to 2^-9, 1.7e-3 rms over a binade) or f16 (2^-12): together 2.0e-3 and 1.2e-3 rms, doubled
+  here. lse: scores are fp32 sums of at most 640 exact products of the query (bf16: exactly; f16: 12 bits kept
+  relative to the head's largest) with the codes, a few 2^-24 of |q| |k| each, and one fp32 sum: 1e-4 absolute.
+* log probabilities and entropy: x - m is one fp32 subtraction, the sums are fp32 over at most 2e5 values added in
+  trees of short chains (under 1e-6 relative): 2e-5 absolute plus 2e-6 of the value.
+"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+TOL_OUT = {torch.bfloat16: 4e-3, torch.float16: 2.4e-3}
+TOL_LSE = 1e-4
+GROUP = 128
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    pkg.build.build()
+    return pkg.glm_cuda.GlmCuda()
+
+
+# ------------------------------------------------------------------ plan
+
+def plan_reference(cached, new, page, free, table, max_tokens):
+    table = table.copy()
+    n_free, stride = len(free), table.shape[1]
+    slots, pos, req, start, taken, status = [], [], [], [0], 0, 0
+    for i, (c, n) in enumerate(zip(cached.tolist(), new.tolist())):
+        if c < 0 or n < 0:
+            status |= 8
+        c, n = max(c, 0), max(n, 0)
+        if -(-(c + n) // page) > stride:
+            status |= 2
+        fresh = {}
+        for col in range(-(-c // page), -(-(c + n) // page)):
+            fresh[col] = int(free[taken]) if taken < n_free else -1
+            if col < stride:
+                table[i, col] = fresh[col]
+            taken += 1
+        for p in range(c, c + n):
+            pg = int(table[i, p // page]) if p // page < stride else -1
+            slots.append(pg * page + p % page if pg >= 0 else -1)
+            pos.append(p)
+            req.append(i)
+        start.append(start[-1] + n)
+    status |= (taken > n_free) * 1 | (start[-1] > max_tokens) * 4
+    cut = lambda v: np.array((v + [-1] * max_tokens)[:max_tokens])  # noqa: E731
+    return dict(slots=cut(slots), positions=cut(pos), token_req=cut(req), token_start=np.array(start),
+                summary=np.array([start[-1], taken, status, 0]), table=table)
+
+
+def run_plan(lib, cached, new, page, free, table, max_tokens, stream=None):
+    d = lambda a, t=np.int32: torch.from_numpy(np.ascontiguousarray(a, dtype=t)).cuda()  # noqa: E731
+    tb = d(table)
+    out = dict(slots=torch.full((max_tokens,), 77, dtype=torch.int64, device="cuda"),
+               positions=torch.full((max_tokens,), 77, dtype=torch.int32, device="cuda"),
+               token_req=torch.full((max_tokens,), 77, dtype=torch.int32, device="cuda"),
+               token_start=torch.full((len(cached) + 1,), 77, dtype=torch.int32, device="cuda"),
+               summary=torch.full((4,), 77, dtype=torch.int32, device="cuda"))
+    lib.kv_plan_async(d(cached), d(new), page, d(free), tb, max_tokens, out["slots"], out["positions"],
+                      out["token_req"], out["token_start"], out["summary"], stream)
+    torch.cuda.synchronize()
+    return dict({k: v.cpu().numpy() for k, v in out.items()}, table=tb.cpu().numpy())
+
+
+def plan_case(seed, n_req, page, top_cached, top_new, spare=3):
+    r = np.random.default_rng(seed)
+    cached = r.integers(0, top_cached + 1, n_req)
+    new = r.integers(0, top_new + 1, n_req)
+    have, want = -(-cached // page), -(-(cached + new) // page)
+    stride = max(1, int(want.max()) + 2)
+    ids = r.permutation(int(want.sum()) + spare)
+    table = np.full((n_req, stride), -1)
+    table[np.arange(stride)[None] < have[:, None]] = ids[: have.sum()]
+    return cached, new, ids[have.sum():], table
+
+
+@pytest.mark.parametrize("n_req,page,top_cached,top_new", [
+    (1, 16, 0, 1), (1, 64, 100, 0), (1, 16, 33, 5000), (7, 1, 5, 5), (33, 64, 200, 1), (1000, 16, 500, 40),
+    (1025, 128, 3000, 3), (16384, 32, 60, 3)])
+def test_plan(lib, n_req, page, top_cached, top_new):
+    cached, new, free, table = plan_case(n_req + page, n_req, page, top_cached, top_new)
+    max_tokens = int(new.sum()) + 6
+    got = run_plan(lib, cached, new, page, free, table, max_tokens)
+    ref = plan_reference(cached, new, page, free, table, max_tokens)
+    for k, v in ref.items():
+        np.testing.assert_array_equal(got[k], v, err_msg=k)
+
+
+def test_plan_reports_what_does_not_fit(lib):
+    cached, new, free, table = plan_case(3, 20, 16, 50, 40)
+    n = int(new.sum())
+    new2 = new.copy()
+    new2[4] = -9
+    cached2 = cached.copy()
+    cached2[5] = -1
+    for c, w, f, tb, m, bits in ((cached, new, free[:5], table, n, 1), (cached, new, free[:0], table, n, 1),
+                                 (cached, new, free, table[:, :3].copy(), n, 2), (cached, new, free, table, n - 11, 4),
+                                 (cached, new, free, table, 0, 4), (cached2, new2, free, table, n, 8)):
+        got, ref = run_plan(lib, c, w, 16, f, tb, m), plan_reference(c, w, 16, f, tb, m)
+        assert ref["summary"][2] & bits
+        for k, v in ref.items():
+            np.testing.assert_array_equal(got[k], v, err_msg=f"{k}, status {bits}")
+
+
+def test_plan_lengths_near_the_integer_limit(lib):
+    """Sums past 2^31 saturate, nothing wraps and nothing outside the arrays is touched."""
+    top = 2**31 - 1
+    cached, new = np.array([top, 0, 5]), np.array([top, top, 2])
+    table = np.full((3, 2), -1)
+    table[2, 0] = 9
+    got = run_plan(lib, cached, new, 16, np.arange(4), table, 40)
+    assert got["summary"][0] == top and got["summary"][2] & 7 == 7
+    np.testing.assert_array_equal(got["token_start"], [0, top, top, top])
+    assert (got["token_req"] == 0).all() and (got["slots"] == -1).all()
+    np.testing.assert_array_equal(got["table"][2], [9, -1])
+
+
+# ------------------------------------------------------------------ cache rows
+
+def quantise(x):
+    """Codes and scales (fp32) of [n, groups] x values as the formula says, in fp32."""
+    with np.errstate(all="ignore"):
+        top = np.abs(x).max(-1, keepdims=True)
+        s = torch.from_numpy((top / np.float32(7)).astype(np.float32)).to(torch.bfloat16).float().numpy()
+        s = np.where(np.isfinite(x).all(-1, keepdims=True), s, np.float32("nan"))
+        v = np.clip(np.rint(x / s), -7, 7)
+    v = np.where((s > 0) & np.isfinite(v), v, 0)
+    return v, s[..., 0]
+
+
+def pool_of(lib, n_pages, kv, rope, page, fill=0):
+    pages = torch.full((n_pages * lib.kv4_page_bytes(kv, rope, page),), fill, dtype=torch.uint8, device="cuda")
+    return pages, lib.kv4_cache(pages, n_pages, kv, rope, page)
+
+
+def pool_rows(pages, slots, kv, rope, page):
+    """Codes (-8..7) and scales of the rows in `slots`, from the pool's bytes."""
+    rb, ng = (kv + rope) // 2, kv // GROUP + 1
+    pb = page * (rb + 2 * ng)
+    slots = slots.long()
+    p, at = slots // page, slots % page
+    b = pages[(p * pb + at * rb)[:, None] + torch.arange(rb, device="cuda")]
+    v = torch.stack([b & 15, b >> 4], -1).flatten(1).int() - 8
+    o = (p * pb + page * rb)[:, None] + 2 * (torch.arange(ng, device="cuda") * page + at[:, None])
+    s = ((pages[o].int() | (pages[o + 1].int() << 8)) << 16).view(torch.float32)
+    return v, s
+
+
+ROW_SHAPES = [(512, 64, 64), (128, 64, 16), (256, 128, 32), (384, 64, 256), (512, 128, 128)]
+
+
+@pytest.mark.parametrize("kv,rope,page", ROW_SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,gap", [(1, 0), (37, 0), (301, 8), (64, 3)])
+def test_rows(lib, kv, rope, page, dtype, n, gap):
+    """Codes and scales are the formula's bit for bit; rows load back; strides that are 16-byte multiples or not."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n * kv + rope)
+    n_pages = n // page + 5
+    pages, cache = pool_of(lib, n_pages, kv, rope, page, fill=0x5A)
+    slots = torch.randperm(n_pages * page, generator=g, device="cuda")[:n]
+    latent = torch.randn(n, kv + gap, generator=g, device="cuda").to(dtype)[:, :kv]
+    peek = (torch.randn(n, rope + gap, generator=g, device="cuda") * 30).to(dtype)[:, gap:]
+    lib.kv4_store_async(cache, latent, peek, slots)
+    v, s = pool_rows(pages, slots, kv, rope, page)
+    rv, rs = quantise(latent.float().cpu().numpy().reshape(n, -1, GROUP))
+    pv, ps = quantise(peek.float().cpu().numpy()[:, None, :])
+    np.testing.assert_array_equal(v.cpu().numpy(), np.concatenate([rv.reshape(n, kv), pv[:, 0]], 1))
+    np.testing.assert_array_equal(s.cpu().numpy(), np.concatenate([rs, ps], 1))
+    # nothing but these rows has changed
+    other = torch.ones(n_pages * page, dtype=torch.bool, device="cuda")
+    other[slots] = False
+    rest = other.nonzero()[:, 0]
+    v2, _ = pool_rows(pages, rest, kv, rope, page)
+    assert (v2[:, 0::2] == 0xA - 8).all() and (v2[:, 1::2] == 0x5 - 8).all()
+    back, back_p = torch.empty(n, kv + gap, dtype=dtype, device="cuda"), torch.empty(n, rope + gap, dtype=dtype, device="cuda")
+    lib.kv4_load_async(cache, slots, back[:, :kv], back_p[:, gap:])
+    np.testing.assert_array_equal(back[:, :kv].float().cpu().numpy(),
+                                  torch.from_numpy((rv * rs[..., None]).reshape(n, kv).astype(np.float32)).to(dtype).float().numpy())
+    np.testing.assert_array_equal(back_p[:, gap:].float().cpu().numpy(),
+                                  torch.from_numpy((pv * ps[..., None])[:, 0].astype(np.float32)).to(dtype).float().numpy())
+
+
+def test_rows_special_values(lib):
+    """Zeros, single values, subnormals, the largest numbers, halves that tie, NaN and infinity."""
+    kv, rope, page = 512, 64, 16
+    x = np.zeros((12, kv), np.float32)
+    x[1, 5] = -3.25
+    x[2, :128] = 1e-45
+    x[2, 128:256] = np.linspace(-2e-38, 2e-38, 128)
+    x[2, 256:384] = np.linspace(-3e-39, 2.9e-39, 128)
+    x[3, :256] = 3.4028235e38
+    x[3, 7] = -3.4028235e38
+    x[4, :128] = np.arange(128) / 16 - 3.5   # quotients on the halves: amax 4.4375 -> not a half; next row is
+    x[5, :128] = np.clip(np.arange(128) / 4 - 16, -7, 7) / 2
+    x[6, 3], x[6, 200] = np.nan, np.inf
+    x[7, 511] = -np.inf
+    x[8] = np.random.default_rng(1).standard_normal(kv) * 1e30
+    x[9] = np.random.default_rng(2).standard_normal(kv) * 1e-30
+    x[10, ::2] = -0.0
+    x[11] = np.random.default_rng(3).integers(-14, 15, kv) * 0.5  # many exact halves
+    p = np.tile(x[:, :rope], 1)
+    pages, cache = pool_of(lib, 2, kv, rope, page)
+    slots = torch.arange(12, device="cuda")
+    lib.kv4_store_async(cache, torch.from_numpy(x).cuda(), torch.from_numpy(p).cuda(), slots)
+    v, s = pool_rows(pages, slots, kv, rope, page)
+    rv, rs = quantise(x.reshape(12, -1, GROUP))
+    pv, ps = quantise(p[:, None, :])
+    np.testing.assert_array_equal(s.cpu().numpy(), np.concatenate([rs, ps], 1))
+    np.testing.assert_array_equal(v.cpu().numpy(), np.concatenate([rv.reshape(12, kv), pv[:, 0]], 1))
+
+
+def test_rows_outside_the_pool_are_left_out(lib):
+    kv, rope, page, n_pages = 128, 64, 16, 3
+    pages, cache = pool_of(lib, n_pages, kv, rope, page, fill=0x11)
+    before = pages.clone()
+    slots = torch.tensor([-1, n_pages * page, 5, -(2**40), 2**40], device="cuda")
+    x = torch.randn(5, kv, device="cuda")
+    lib.kv4_store_async(cache, x, torch.randn(5, rope, device="cuda"), slots)
+    rows = torch.tensor([5], device="cuda")
+    v, _ = pool_rows(pages, rows, kv, rope, page)
+    assert not (v == 0x1 - 8).all()
+    changed = (pages != before).nonzero()[:, 0]
+    assert len(changed) <= (kv + rope) // 2 + 2 * (kv // GROUP + 1)
+    a, b = torch.full((5, kv), 9.0, device="cuda"), torch.full((5, rope), 9.0, device="cuda")
+    lib.kv4_load_async(cache, slots, a, b)
+    for i in (0, 1, 3, 4):
+        assert (a[i] == 0).all() and (b[i] == 0).all()
+    assert (a[2] != 0).any()
+    lib.kv4_store_async(cache, x[:0], torch.empty(0, rope, device="cuda"), slots[:0])  # no rows: no launch
+
+
+# ------------------------------------------------------------------ attention
+
+def attention_reference(pages, kv, rope, page, n_pages, q, table, row_req, row_pos, scale):
+    """64 bits, one row at a time."""
+    n, heads = q.shape[:2]
+    out = torch.zeros(n, heads, kv, dtype=torch.float64, device="cuda")
+    lse = torch.full((n, heads), -float("inf"), dtype=torch.float64, device="cuda")
+    for r in range(n):
+        req, pos = int(row_req[r]), int(row_pos[r])
+        if not 0 <= req < table.shape[0] or pos < 0:
+            continue
+        t = torch.arange(min(pos + 1, table.shape[1] * page), device="cuda")
+        ids = table[req].long()[t // page]
+        ok = (ids >= 0) & (ids < n_pages)
+        if not bool(ok.any()):
+            continue
+        v, s = pool_rows(pages, (ids * page + t % page)[ok], kv, rope, page)
+        k = torch.cat([(v[:, :kv].double().unflatten(1, (-1, GROUP)) * s[:, :-1, None].double()).flatten(1),
+                       v[:, kv:].double() * s[:, -1:].double()], 1)
+        x = scale * (q[r].double() @ k.T)
+        lse[r] = torch.logsumexp(x, 1)
+        out[r] = torch.softmax(x, 1) @ k[:, :kv]
+    return out, lse
+
+
+def attention_case(lib, seed, kv, rope, page, lens, per_req, heads, dtype, q_std=1.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    r = np.random.default_rng(seed)
+    held = [-(-n // page) for n in lens]
+    n_pages = sum(held) + 2
+    ids = r.permutation(n_pages)
+    table = np.full((len(lens), max(max(held), 1)), -1)
+    table[np.arange(table.shape[1])[None] < np.array(held)[:, None]] = ids[: sum(held)]
+    pages, cache = pool_of(lib, n_pages, kv, rope, page)
+    n = n_pages * page
+    lib.kv4_store_async(cache, torch.randn(n, kv, generator=g, device="cuda"), torch.randn(n, rope, generator=g, device="cuda"),
+                        torch.arange(n, device="cuda"))
+    rows = len(lens) * per_req
+    q = (q_std * torch.randn(rows, heads, kv + rope, generator=g, device="cuda")).to(dtype)
+    pos = [max(-1, n - per_req + j) for n in lens for j in range(per_req)]
+    i32 = lambda a: torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")  # noqa: E731
+    return dict(pages=pages, cache=cache, n_pages=n_pages, q=q, table=i32(table),
+                row_req=i32(np.arange(rows) // per_req), row_pos=i32(pos), scale=1.0 / 16.0, kv=kv, rope=rope, page=page)
+
+
+def run_attention(lib, c, out=None, stream=None, want_lse=True):
+    n, heads = c["q"].shape[:2]
+    if out is None:
+        out = torch.full((n, heads, c["kv"]), 7.0, dtype=c["q"].dtype, device="cuda")
+    lse = torch.full((n, heads), 7.0, device="cuda") if want_lse else None
+    ws = torch.full((lib.mla4_workspace_bytes(n, heads, c["kv"]),), 0xCD, dtype=torch.uint8, device="cuda")
+    lib.mla4_attention_async(c["cache"], c["q"], c["table"], c["row_req"], c["row_pos"], c["scale"], out, lse, ws, stream)
+    torch.cuda.synchronize()
+    return out, lse
+
+
+def check_attention(lib, c, **kw):
+    out, lse = run_attention(lib, c, **kw)
+    ref, ref_lse = attention_reference(c["pages"], c["kv"], c["rope"], c["page"], c["n_pages"], c["q"], c["table"],
+                                       c["row_req"], c["row_pos"], c["scale"])
+    none = torch.isinf(ref_lse)
+    assert torch.equal(none, torch.isinf(lse)) and (lse[none] < 0).all()
+    assert (out[none] == 0).all()
+    for r in range(out.shape[0]):
+        for h in range(out.shape[1]):
+            if not none[r, h]:
+                err = float((out[r, h].double() - ref[r, h]).norm() / ref[r, h].norm())
+                assert err <= TOL_OUT[out.dtype], (r, h, err)
+    if not none.all():
+        assert float((lse.double() - ref_lse)[~none].abs().max()) <= TOL_LSE
+    return out, lse
+
+
+@pytest.mark.parametrize("kv,rope,page,heads", [
+    (512, 64, 64, 20), (512, 64, 16, 5), (128, 64, 32, 4), (256, 128, 256, 8), (384, 64, 128, 17), (512, 128, 64, 24),
+    (512, 64, 64, 25), (512, 64, 32, 1), (128, 128, 16, 48), (512, 64, 64, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention(lib, kv, rope, page, heads, dtype):
+    """Ragged lengths around tile and page ends, one position and none, two query tokens a request."""
+    lens = [1, 0, 2, 63, 64, 65, 127, 129, 255, 700, 1, 1031]
+    check_attention(lib, attention_case(lib, kv + page + heads, kv, rope, page, lens, 2, heads, dtype))
+
+
+@pytest.mark.parametrize("length", [1, 15, 16, 17, 64, 100, 1024, 5000, 40001])
+def test_attention_of_one_request(lib, length):
+    check_attention(lib, attention_case(lib, length, 512, 64, 64, [length], 1, 20, torch.bfloat16))
+
+
+def test_attention_of_nothing(lib):
+    c = attention_case(lib, 5, 512, 64, 64, [0, 0, 0], 1, 20, torch.bfloat16)
+    out, lse = check_attention(lib, c)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    c["q"] = c["q"][:0]
+    c["row_req"], c["row_pos"] = c["row_req"][:0], c["row_pos"][:0]
+    ws = torch.empty(16, dtype=torch.uint8, device="cuda")
+    lib.mla4_attention_async(c["cache"], c["q"], c["table"], c["row_req"], c["row_pos"], 1.0, c["q"][..., :512], None, ws)
+
+
+def test_attention_many_short_rows(lib):
+    """More rows than CTAs, most of them shorter than a tile."""
+    lens = [(i * 37) % 90 for i in range(700)]
+    check_attention(lib, attention_case(lib, 8, 128, 64, 16, lens, 1, 3, torch.bfloat16))
+
+
+def test_attention_strides_streams_and_repeats(lib):
+    """q and out with gaps (not 16-byte multiples), another stream, no lse; two runs agree bit for bit."""
+    c = attention_case(lib, 21, 512, 64, 64, [300, 77, 1500], 1, 20, torch.bfloat16)
+    out, lse = check_attention(lib, c)
+    n, h = c["q"].shape[:2]
+    wide = torch.empty(n, h + 1, 576 + 3, dtype=torch.bfloat16, device="cuda")
+    wide[:, :h, 1:577] = c["q"]
+    c2 = dict(c, q=wide[:, :h, 1:577])
+    gap = torch.full((n, h, 512 + 5), 3.0, dtype=torch.bfloat16, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    run_attention(lib, c2, out=gap[..., 2:514], stream=side.cuda_stream, want_lse=False)
+    assert torch.equal(gap[..., 2:514], out)
+    assert (gap[..., :2] == 3).all() and (gap[..., 514:] == 3).all()
+    out2, lse2 = run_attention(lib, c)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+def test_attention_does_not_see_what_is_masked(lib):
+    """NaN scales, infinite scales and any codes past a request's length, in unlisted pages and in pages outside
+    the pool leave the result as it is; requests that are not there and too long positions are cut."""
+    c = attention_case(lib, 33, 512, 64, 16, [50, 20, 130, 33], 1, 20, torch.bfloat16)
+    out, lse = check_attention(lib, c)
+    page, pb = 16, lib.kv4_page_bytes(512, 64, 16)
+    pool = c["pages"].view(c["n_pages"], pb)
+    seen = torch.zeros(c["n_pages"], page, dtype=torch.bool, device="cuda")
+    for r in range(4):
+        t = torch.arange(int(c["row_pos"][r]) + 1, device="cuda")
+        seen[c["table"][r].long()[t // page], t % page] = True
+    scales = pool[:, page * 288:].unflatten(1, (5, page, 2))
+    for bits in (0x7FC0, 0x7F80, 0xFF80, 0xFFFF):
+        two = torch.tensor([bits & 255, bits >> 8], dtype=torch.uint8, device="cuda")
+        scales.copy_(torch.where(seen[:, None, :, None], scales, two))
+        out2, lse2 = run_attention(lib, c)
+        assert torch.equal(out, out2) and torch.equal(lse, lse2), hex(bits)
+    # a seen NaN does come through, for its row alone
+    c["table"][1, 1], keep = -1, int(c["table"][1, 1])  # positions 16..19 of request 1 are not seen
+    check_attention(lib, c)
+    c["table"][1, 1] = c["n_pages"]
+    check_attention(lib, c)
+    c["table"][1, 1] = 2**31 - 1
+    check_attention(lib, c)
+    c["table"][1, 1] = keep
+    c["row_req"][0], c["row_req"][3] = -1, 4
+    out3, lse3 = check_attention(lib, c)
+    assert (out3[0] == 0).all() and (out3[3] == 0).all()
+    c["row_req"][0], c["row_req"][3] = 0, 3
+    c["row_pos"][2] = 2**31 - 1  # past the block table: its whole row
+    c["table"][2, -1] = c["table"][2, 0]
+    scales[seen.logical_not().nonzero()[:, 0], :, seen.logical_not().nonzero()[:, 1]] = 0
+    check_attention(lib, c)
+    scales[int(c["table"][3, 0]), 2, 4] = torch.tensor([0xC0, 0x7F], dtype=torch.uint8, device="cuda")
+    out4, lse4 = run_attention(lib, c)
+    assert torch.isnan(lse4[3]).all() and torch.isnan(out4[3]).all(-1).all() and not torch.isnan(out4[:3]).any()
+
+
+def test_attention_of_peaked_and_flat_scores(lib):
+    """One position far above a long flat tail whose weight still counts; scores of hundreds; a query of zeros,
+    one with values of very different size, one with a NaN and one with an infinity."""
+    c = attention_case(lib, 44, 512, 64, 64, [30000, 9000, 300, 300, 300, 300], 1, 4, torch.bfloat16, q_std=0.05)
+    # position 0 of request 0: its row's code pattern as the query, so that it stands out by about 12
+    v, s = pool_rows(c["pages"], c["table"][0, :1] * 64, 512, 64, 64)
+    k = torch.cat([(v[:, :512].float().unflatten(1, (4, 128)) * s[:, :4, None]).flatten(1), v[:, 512:].float() * s[:, 4:]], 1)[0]
+    c["q"][0] = (k * (12 * 16 / float(k @ k))).to(torch.bfloat16)
+    c["q"][1] *= 2000
+    c["q"][2] = 0
+    c["q"][3, :, ::2] *= 1e-6
+    check_attention(lib, c)
+    c["q"][4, 1, 3], c["q"][5, 2, 70] = float("nan"), float("inf")
+    out, lse = run_attention(lib, c)
+    for r, h in ((4, 1), (5, 2)):
+        assert torch.isnan(out[r, h]).all() and torch.isnan(lse[r, h])
+    bad = torch.isnan(out).any(-1)
+    assert int(bad.sum()) == 2
+
+
+def test_attention_offsets_past_32_bits(lib):
+    """A pool of over 4 GB whose pages in use lie at its end."""
+    kv, rope, page, n_pages = 512, 64, 64, 260000
+    pb = lib.kv4_page_bytes(kv, rope, page)
+    assert pb * n_pages > 2**32
+    pages = torch.empty(pb * n_pages, dtype=torch.uint8, device="cuda")
+    cache = lib.kv4_cache(pages, n_pages, kv, rope, page)
+    ids = torch.arange(n_pages - 20, n_pages, device="cuda")
+    slots = (ids[:, None] * page + torch.arange(page, device="cuda")).flatten()
+    x, p = torch.randn(len(slots), kv, device="cuda"), torch.randn(len(slots), rope, device="cuda")
+    lib.kv4_store_async(cache, x, p, slots)
+    a, b = torch.empty_like(x), torch.empty_like(p)
+    lib.kv4_load_async(cache, slots, a, b)
+    assert float((a - x).norm() / x.norm()) < 0.2 and float((b - p).norm() / p.norm()) < 0.2
+    c = dict(pages=pages, cache=cache, n_pages=n_pages, q=torch.randn(2, 20, kv + rope, device="cuda").bfloat16(),
+             table=ids.int().view(2, 10).contiguous(), row_req=torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+             row_pos=torch.tensor([639, 400], dtype=torch.int32, device="cuda"), scale=1 / 16.0, kv=kv, rope=rope, page=page)
+    check_attention(lib, c)
+
+
+# ------------------------------------------------------------------ log probabilities
+
+def logprobs_reference(x, target, k):
+    x = x.double()
+    m = x.amax(1, keepdim=True)
+    dead = torch.isneginf(m[:, 0])
+    d = torch.where(dead[:, None], -float("inf"), x - m)  # m + ln sum would round ln sum away where |m| is large
+    log_l = torch.exp(d).sum(1, keepdim=True).log()
+    lp = d - torch.where(dead[:, None], 0.0, log_l)
+    e = torch.where(lp == -float("inf"), 0.0, torch.exp(lp) * lp).sum(1)
+    ids = torch.argsort(-x, dim=1, stable=True)[:, :k]
+    v = x.gather(1, ids)
+    pad = k - ids.shape[1]
+    top = torch.where(v > -float("inf"), ids, -1)
+    top = torch.cat([top, top.new_full((len(x), pad), -1)], 1)
+    tl = torch.cat([lp.gather(1, ids), v.new_full((len(x), pad), -float("inf"))], 1)
+    tl = torch.where(top < 0, -float("inf"), tl)
+    t = target.long()
+    ok = (t >= 0) & (t < x.shape[1])
+    own = torch.where(ok, lp.gather(1, t.clamp(0, x.shape[1] - 1)[:, None])[:, 0], -float("inf"))
+    return torch.where(dead, -float("inf"), own), torch.where(dead, 0.0, -e), top, tl
+
+
+def run_logprobs(lib, x, target, k, stream=None):
+    n = x.shape[0]
+    lp, en = torch.full((n,), 5.0, device="cuda"), torch.full((n,), 5.0, device="cuda")
+    ids = torch.full((n, k), 55, dtype=torch.int32, device="cuda") if k else None
+    tl = torch.full((n, k), 5.0, device="cuda") if k else None
+    lib.logprobs_async(x, target, lp, en, ids, tl, stream)
+    torch.cuda.synchronize()
+    return lp, en, ids, tl
+
+
+def close(a, b):
+    a, b = a.double(), b.double()
+    assert torch.equal(torch.isinf(a), torch.isinf(b)) and not torch.isnan(a).any()
+    f = ~torch.isinf(b)
+    assert ((a - b)[f].abs() <= 2e-5 + 2e-6 * b[f].abs()).all(), float((a - b)[f].abs().max())
+
+
+def check_logprobs(lib, x, target, k):
+    lp, en, ids, tl = run_logprobs(lib, x, target, k)
+    rlp, ren, rids, rtl = logprobs_reference(x, target, k)
+    close(lp, rlp)
+    close(en, ren)
+    if k:
+        assert torch.equal(ids.long(), rids)
+        close(tl, rtl)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (3, 7, 32), (2, 31, 5), (5, 33, 32), (1, 1000, 20), (300, 515, 8),
+                                       (1, 154880, 5), (40, 154880, 32), (160, 20001, 1), (2, 50257, 0)])
+def test_logprobs(lib, dtype, n, vocab, k):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(vocab + k)
+    x = (3 * torch.randn(n, vocab, generator=g, device="cuda")).to(dtype)  # 16-bit types: many ties
+    target = torch.randint(0, vocab, (n,), generator=g, device="cuda", dtype=torch.int32)
+    check_logprobs(lib, x, target, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logprobs_orders_and_ties(lib, dtype):
+    """Ascending, descending, constant, two-valued rows, zeros of both signs; 20000 values over one CTA or several."""
+    n = 20000
+    base = torch.linspace(-9, 9, n, device="cuda")
+    zeros = torch.zeros(n, device="cuda")
+    zeros[::3] = -0.0
+    two = (torch.arange(n, device="cuda") % 977 == 5).float()
+    rows = torch.stack([base, base.flip(0), torch.full_like(base, 2.5), two, zeros, -two, base.roll(7001), 1e4 + base])
+    target = torch.arange(8, dtype=torch.int32, device="cuda") * 2000
+    check_logprobs(lib, rows.to(dtype), target, 32)
+    check_logprobs(lib, rows.to(dtype).repeat(40, 1), target.repeat(40), 13)
+    check_logprobs(lib, rows[:1].to(dtype), target[:1], 32)
+
+
+def test_logprobs_masks_and_values_that_are_no_numbers(lib):
+    n, inf = 5003, float("inf")
+    g = torch.Generator(device="cuda")
+    g.manual_seed(9)
+    x = torch.randn(9, n, generator=g, device="cuda")
+    x[0, torch.rand(n, generator=g, device="cuda") < 0.9] = -inf
+    x[1] = -inf
+    x[2] = -inf
+    x[2, 4999] = -3.0                 # one token left
+    x[3, :] = torch.finfo(torch.float32).min  # every token at the type's lowest
+    x[4, :] = -inf
+    x[4, [5, 4000, 17]] = torch.tensor([1.0, 2.0, 1.0], device="cuda")
+    x[5, 10] = torch.finfo(torch.float32).min
+    target = torch.tensor([int(x[0].argmax()), 3, 4999, 8, 17, 10, -1, n, 2], dtype=torch.int32, device="cuda")
+    check_logprobs(lib, x, target, 32)
+    x[6, 100], x[7, 200], x[8, 0] = float("nan"), inf, float("nan")
+    lp, en, ids, tl = run_logprobs(lib, x, target, 4)
+    for r in (6, 7, 8):
+        assert torch.isnan(en[r])
+    assert torch.isneginf(lp[6]) and torch.isneginf(lp[7])  # targets outside the vocabulary
+    assert torch.isnan(lp[8])
+    assert int(ids[7, 0]) == 200
+    y = torch.where(torch.isnan(x), -inf, x)
+    assert torch.equal(ids.long(), logprobs_reference(torch.where(torch.isinf(y) & (y > 0), 1e30, y), target, 4)[2])
+
+
+def test_logprobs_strides_alignment_and_streams(lib):
+    """Rows that start anywhere, gaps between them, another stream; parts of the outputs left out."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(10)
+    for dtype in (torch.float32, torch.bfloat16):
+        wide = torch.randn(6, 3007, generator=g, device="cuda").to(dtype)
+        for lo in range(0, 9):
+            x = wide[:, lo: lo + 2990]
+            check_logprobs(lib, x, torch.full((6,), 2989, dtype=torch.int32, device="cuda"), 7)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    t = torch.zeros(6, dtype=torch.int32, device="cuda")
+    a, b = run_logprobs(lib, x, t, 7), run_logprobs(lib, x, t, 7, side.cuda_stream)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    ent = torch.empty(6, device="cuda")
+    lib.logprobs_async(x, entropy=ent)
+    torch.cuda.synchronize()
+    assert torch.equal(ent, run_logprobs(lib, x, t, 0)[1])
+
+
+# ------------------------------------------------------------------ refusals
+
+def test_wrapper_refuses_wrong_tensors(lib):
+    z = lambda *s, t=torch.int32: torch.zeros(*s, dtype=t, device="cuda")  # noqa: E731
+    with pytest.raises(ValueError):
+        lib.kv_plan_async(z(4, t=torch.int64), z(4), 16, z(3), z(4, 2), 0, z(0, t=torch.int64), z(0), z(0), z(5), z(4))
+    with pytest.raises(ValueError):
+        lib.kv_plan_async(z(4), z(3), 16, z(3), z(4, 2), 0, z(0, t=torch.int64), z(0), z(0), z(5), z(4))
+    with pytest.raises(ValueError):
+        lib.kv4_cache(z(100, t=torch.uint8), 1, 512, 64, 64)
+    _, cache = pool_of(lib, 1, 128, 64, 16)
+    with pytest.raises(ValueError):
+        lib.kv4_store_async(cache, torch.zeros(2, 128, device="cuda"), torch.zeros(2, 64, device="cuda").half(), z(2, t=torch.int64))
+    with pytest.raises(ValueError):
+        lib.kv4_store_async(cache, torch.zeros(2, 256, device="cuda")[:, ::2], torch.zeros(2, 64, device="cuda"), z(2, t=torch.int64))
+    with pytest.raises(ValueError):
+        lib.logprobs_async(torch.zeros(2, 10, device="cuda", dtype=torch.float64))
+    with pytest.raises(ValueError):
+        lib.logprobs_async(torch.zeros(2, 10, device="cuda"), z(2), torch.zeros(3, device="cuda"))
