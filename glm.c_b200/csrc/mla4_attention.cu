@@ -10,9 +10,47 @@
 // A position whose page is not in the pool is not seen. A row that sees
 // nothing gives zeros and lse = -inf.
 //
-// Simple form: one CTA per (row, head), a warp per position with the running
-// maximum and sum of the softmax, the warps joined at the end.
+// Work split. The (row, head block) items' tiles of 64 positions form one
+// list, of which every CTA (one per SM) takes an equal consecutive part,
+// wherever that begins and ends; an item that lies in several parts is joined
+// from their partial sums by a second small kernel, in a fixed order.
+//
+// Products. Both run on the tensor cores as m16n8k16 f16 with fp32
+// accumulation, positions (first product) or latents (second) as rows and
+// heads as columns, up to 24 of them. The cached operand goes from the packed
+// words in shared memory straight into fragments: four bits put into the
+// mantissa of 1024 are 1024 + u (or 1024 + 16 u), and one packed operation
+// makes it v = u - 8, exactly, two values at a time. The query is exact in f16
+// after a power of two per head; the probabilities are rounded to f16 (11
+// bits, relative to the tile's largest).
+// At 20 heads a position takes 12.75 of these instructions, 25.5 clocks of an
+// SM at the measured 0.50 a clock, against 13.3 clocks for its 298 bytes from
+// memory: the tensor pipe is the bound. Measured on the way here: the e4m3
+// form of the instruction is no faster (it is unpacked to f16 first, 3.6 times
+// the instructions); int8 does twice the products a clock but needs two digits
+// for either operand. tcgen05 would need the cached operand written to shared
+// memory as bytes and read back for each product, by count 17 to 22 clocks a
+// position of shared-memory traffic.
+//
+// Scales. A position has one scale per 128 latents. The first product ends at
+// each group and is multiplied into the score; for the second the scale goes
+// into the probability, in one version per group: p * s / ref_g.
+//
+// References. p = e^(x - R) with R the item's running reference per head, not
+// its maximum: R moves up to a unit's maximum when that exceeds it by more
+// than 4, so that p stays below 55 and most units leave R as it is; ref_g, a
+// power of two, moves likewise when a scale exceeds 16 ref_g. The second
+// product then accumulates in the tensor core's own accumulators from unit to
+// unit. A unit's references follow from its predecessor's, in order, whichever
+// warps run them: results do not depend on timing.
+//
+// Roles. Warp 16 copies tiles of 64 positions into a ring in shared memory
+// (cp.async.bulk, completion on mbarriers). Warps 0-7 take a unit of 32
+// positions each in turn: scores, references, the probabilities in f16. Warps
+// 8-15 own 64 latents each: the second product of every unit.
+
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -27,7 +65,15 @@
 namespace glmq {
 namespace {
 
-constexpr int kAtWarps = 8, kAtThreads = kAtWarps * 32;
+constexpr int kTile = 64;                 // positions that are copied together
+constexpr int kUnit = 32;                 // positions that a score warp takes together
+constexpr int kScoreWarps = 8, kSumWarps = 8;
+constexpr float kRaise = 4.f, kRaiseScale = 16.f;
+constexpr int kProducer = kScoreWarps + kSumWarps;
+constexpr int kAtThreads = 640;           // warpgroups: two of scores, two of sums, one of which a warp copies
+constexpr int kMaxCtas = 148;             // one per SM of a B200; the workspace is laid out for them
+constexpr int kMaxBlockHeads = 24;
+constexpr int kMaxStages = 8;
 
 struct Mla4Args {
     Kv4Shape sh;
@@ -38,75 +84,993 @@ struct Mla4Args {
     const int32_t* table;
     int table_stride, n_req;
     const int32_t *row_req, *row_pos;
-    int n_heads;
+    int n_rows, n_heads;
+    int blocks, block_heads;  // head blocks, heads in each (the last may have fewer)
     float scale;
     void* out;
     long long out_row, out_head;
     float* lse;
+    unsigned char* ws;
+    int stages;
+    int vec;  // q and out rows start on 16-byte boundaries
 };
 
-__device__ __forceinline__ float load_q(const void* q, long long i, int type) {
-    if (type == GLM_CUDA_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(q)[i]);
-    return __half2float(static_cast<const __half*>(q)[i]);
+// ------------------------------------------------------------ workspace
+
+// status word; what is to be joined; every CTA's two partial sums: [0] of an
+// item that began in an earlier CTA's part, [1] of one that goes on in a later
+// one. With at most kMaxCtas items the joins are listed by item, otherwise by
+// the CTA that an item begins in and goes on from (at most one a CTA).
+struct Join {
+    int item, first, last;  // the item and the CTAs it begins and ends in; first = -1: it lies in one
+};
+
+struct WsLayout {
+    size_t joins, stats, sums, bytes;
+    __host__ __device__ WsLayout(int block_heads, int kv_lora) {
+        joins = 16;
+        stats = joins + kMaxCtas * sizeof(Join);
+        sums = (stats + (size_t)kMaxCtas * 2 * block_heads * 8 + 15) / 16 * 16;
+        bytes = sums + (size_t)kMaxCtas * 2 * block_heads * kv_lora * 4;
+    }
+};
+
+__host__ __device__ inline int head_blocks(int n_heads) { return (n_heads + kMaxBlockHeads - 1) / kMaxBlockHeads; }
+__host__ __device__ inline int heads_per_block(int n_heads) {
+    const int b = head_blocks(n_heads);
+    return (n_heads + b - 1) / b;
 }
 
-__global__ void __launch_bounds__(kAtThreads) mla4_attention_kernel(Mla4Args a, int type) {
-    __shared__ float q[640], acc_s[kAtWarps][512], m_s[kAtWarps], l_s[kAtWarps];
-    pdl_enter();
-    const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int dim = a.sh.kv_lora + a.sh.rope;
-    for (int i = threadIdx.x; i < dim; i += kAtThreads) q[i] = load_q(a.q, row * a.q_row + h * a.q_head + i, type);
-    __syncthreads();
-    const int req = a.row_req[row];
-    long long len = req >= 0 && req < a.n_req ? (long long)a.row_pos[row] + 1 : 0;
-    len = min(len, (long long)a.table_stride * a.sh.page);
-    float m = -INFINITY, l = 0.f, acc[16] = {};
-    for (long long t = warp; t < len; t += kAtWarps) {
-        const int page = a.table[(size_t)req * a.table_stride + t / a.sh.page], at = (int)(t % a.sh.page);
-        if (page < 0 || page >= a.n_pages) continue;
-        const unsigned char* p = a.pages + (size_t)page * a.sh.page_bytes();
-        const __nv_bfloat16* sc = reinterpret_cast<const __nv_bfloat16*>(p + (size_t)a.sh.page * a.sh.row_bytes());
-        float x = 0.f, v[20];
+// -------------------------------------------------------- shared memory
+
+template <int NT>
+struct Smem {
+    static constexpr int kScaleBytes = kKv4MaxGroups * kUnit * 4, kRatioBytes = 4 * kUnit * 2;
+    static constexpr int kProbBytes = 4 * NT * 8 * kUnit * 2;  // [group][n tile][8 heads][32 positions]
+    static constexpr int kStats = 16 * NT + 8;                 // R [8 NT], l [8 NT], ref [4], moved, pad
+    int qf, query, scratch, probs, stats, chain, ring, stage, bytes;
+    __host__ __device__ Smem(const Kv4Shape& sh, int stages) {
+        const int words = (sh.kv_lora + sh.rope) / 32;  // words of 8 values that a lane-in-quad has of a row
+        int o = 0;
+        qf = o;      // two items' queries: [word][n tile][lane] 16 bytes, the fragments of the word's two steps, ...
+        query = words * NT * 512 + 8 * NT * 4;  // ... then each column's factor [8 NT]
+        o += 2 * query;
+        scratch = o; // per score warp: scales, ratios
+        o += kScoreWarps * (kScaleBytes + kRatioBytes);
+        probs = o;   // per score warp
+        o += kScoreWarps * kProbBytes;
+        stats = o;   // per score warp
+        o += kScoreWarps * kStats * 4;
+        chain = o;   // the item's references after the last unit: R [8 NT], ref [4]
+        o += (8 * NT + 4) * 4;
+        o = (o + 127) / 128 * 128;
+        ring = o;
+        stage = (kTile * (sh.row_bytes() + 2 * sh.groups()) + 127) / 128 * 128;
+        bytes = ring + stages * stage;
+    }
+};
+
+// ------------------------------------------------------------- helpers
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                        const float (&c)[4]) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%11,%12,%13};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// (w & mask) | 0x6400 in both halves, one operation.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
+    return r;
+}
+
+// Eight codes to f16 values: v[i] holds those of nibbles i (low half) and i + 4.
+__device__ __forceinline__ void unpack8(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t x = w >> 8;
+    const uint32_t p[4] = {and_or(w, 0x000f000fu), and_or(w, 0x00f000f0u), and_or(x, 0x000f000fu), and_or(x, 0x00f000f0u)};
 #pragma unroll
-        for (int i = 0; i < 20; ++i) {
-            const int e = i * 32 + lane;
-            v[i] = 0.f;
-            if (e >= dim) continue;
-            const unsigned b = p[(size_t)at * a.sh.row_bytes() + e / 2];
-            const int g = min(e / kKv4Group, a.sh.groups() - 1);
-            v[i] = (float)((int)((e & 1 ? b >> 4 : b) & 15u) - 8) * __bfloat162float(sc[g * a.sh.page + at]);
-            x += q[e] * v[i];
+    for (int i = 0; i < 4; ++i)
+        if (i & 1)  // 1024 + 16 u: / 16, - 72
+            asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(v[i]) : "r"(p[i]), "r"(0x2c002c00u), "r"(0xd480d480u));
+        else        // 1024 + u: - 1032
+            asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(v[i]) : "r"(p[i]), "r"(0xe408e408u));
+}
+
+// e^d for a difference d <= 0. Scores stay in natural units: differences are
+// formed before the product with log2 e, so that scores of hundreds lose nothing.
+__device__ __forceinline__ float exp_of(float d) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(d * 1.4426950408889634f));
+    return y;
+}
+
+// Registers of the calling warpgroup's threads. The launch has 96 for each of
+// 640 threads, 5 x 96 = 480 over a thread of every group; the groups' shares
+// are 32 + 4 x 112.
+constexpr int kCopyRegs = 32, kMathRegs = 112;
+static_assert(kCopyRegs + 4 * kMathRegs <= 5 * 96, "more registers than the launch has");
+template <int kRegs>
+__device__ __forceinline__ void shrink_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void grow_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegs));
+}
+
+// A bounded wait whose outcome is the whole warp's.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+}
+
+// Positions that row `row` sees.
+__device__ __forceinline__ long long row_length(const Mla4Args& a, int row) {
+    const int req = a.row_req[row], pos = a.row_pos[row];
+    if (req < 0 || req >= a.n_req || pos < 0) return 0;
+    const long long len = (long long)pos + 1, most = (long long)a.table_stride * a.sh.page;
+    return len < most ? len : most;
+}
+
+// A row of no positions has one tile, in which it sees nothing.
+__device__ __forceinline__ int tiles_of(long long len) { return len > kTile ? (int)((len + kTile - 1) / kTile) : 1; }
+
+// A place in the ring of stages and the phase its barriers are in.
+struct Place {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void forward(int tiles, int stages) {
+        for (stage += tiles; stage >= stages; stage -= stages) phase ^= 1u;
+    }
+};
+
+// The consecutive pieces of items that a CTA's part of the tile list is made of.
+struct Walk {
+    const Mla4Args& a;
+    int item, tile;   // next piece: item, first tile in it
+    long long left;   // tiles of the part still to come
+    int row, block, first, end, n;  // this piece: tiles [first, end) of the item's n
+    long long len;
+    __device__ Walk(const Mla4Args& args, int item0, int tile0, long long tiles)
+        : a(args), item(item0), tile(tile0), left(tiles) {}
+    __device__ bool next() {
+        if (left <= 0) return false;
+        row = item / a.blocks;
+        block = item - row * a.blocks;
+        len = row_length(a, row);
+        n = tiles_of(len);
+        first = tile;
+        end = (long long)(n - first) < left ? n : first + (int)left;
+        left -= end - first;
+        item += 1;
+        tile = 0;
+        return true;
+    }
+};
+
+// ----------------------------------------------------------- the query
+
+// The item's query as B fragments: head c of the block is column c of the
+// products. A power of two brings the head's largest value to [2^14, 2^15), so
+// that a bf16 value is exact in f16 down to 2^-30 of it. A word's two steps
+// meet its nibbles (0, 4), (1, 5) and (2, 6), (3, 7).
+template <int NT, bool kBf16>
+__device__ __forceinline__ void load_query(const Mla4Args& a, int row, int block, unsigned char* qf, int warp, int lane) {
+    const int chunks = (a.sh.kv_lora + a.sh.rope) / 8;  // at most 80
+    const int h0 = block * a.block_heads;
+    float* factor = reinterpret_cast<float*>(qf + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
+    // warp w has the heads w, w + 8, ...: all their loads go out before the first is used
+    static_assert(kScoreWarps == 8, "a head of each n tile to a warp");
+    uint32_t raw[NT][3][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = 8 * n + warp;
+        const bool live = c < a.block_heads && h0 + c < a.n_heads;
+        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (long long)row * a.q_row + (long long)(h0 + c) * a.q_head;
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            const int ch = u * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[n][u][i] = 0u;
+            if (live && ch < chunks) {
+                if (a.vec) {
+                    const uint4 r = __ldg(reinterpret_cast<const uint4*>(q + ch * 8));
+                    raw[n][u][0] = r.x;
+                    raw[n][u][1] = r.y;
+                    raw[n][u][2] = r.z;
+                    raw[n][u][3] = r.w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) raw[n][u][i >> 1] |= (uint32_t)q[ch * 8 + i] << (16 * (i & 1));
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = 8 * n + warp;
+        float v[3][8];
+        unsigned top = 0u;
+#pragma unroll
+        for (int u = 0; u < 3; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = raw[n][u][i >> 1] >> (16 * (i & 1)) & 0xffffu;
+                v[u][i] = kBf16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half((uint16_t)b));
+                top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
+            }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const bool bad = top >= 0x7f800000u;
+        // 2^k with top * 2^k in [2^14, 2^15); a head of zeros or of values below 2^-103 stays small
+        int k = 127 + 14 - (int)(top >> 23);
+        k = min(max(k, -120), 117);
+        const float up = __uint_as_float((unsigned)(127 + k) << 23);
+#pragma unroll
+        for (int u = 0; u < 3; ++u) {
+            const int ch = u * 32 + lane;
+            if (ch >= chunks) continue;
+            uint32_t f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 h = __floats2half2_rn(bad ? 0.f : v[u][i] * up, bad ? 0.f : v[u][i + 4] * up);
+                f[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            // chunk ch is word ch % 8 of its 64 values: lane-in-quad (ch % 8) / 2, the first or second word it loads
+            const int word = 2 * (ch >> 3) + (ch & 1), to = 4 * (c & 7) + ((ch & 7) >> 1);
+            *reinterpret_cast<uint4*>(qf + ((word * NT + (c >> 3)) * 32 + to) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
+        }
+        if (lane == 0)
+            factor[c] = bad ? __uint_as_float(0x7fc00000u) : __uint_as_float((unsigned)(127 - k) << 23) * a.scale;
+    }
+}
+
+// 8-byte piece at which a head row of 32 probabilities keeps piece u: off one
+// another's banks both where 16 lanes write four pieces of four rows and where
+// they read them.
+__device__ __forceinline__ int swizzled(int u, int row) { return u ^ (4 * (row >> 1 & 1)); }
+
+// -------------------------------------------------------------- scores
+
+// One unit's scores and probabilities. Lane (g, t) holds positions 8 j + g
+// (j = 0..3: row g or g + 8 of product j / 2) of heads 2 t and 2 t + 1 of each
+// n tile. Returns false when a wait gave up.
+//   rows    the unit's codes; scales: of position `lane`, scale_step bytes from group to group
+//   query   the item's fragments and factors
+//   seen    its positions that the row sees
+//   first   the item's first unit in this part
+template <int NT>
+__device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm, const Smem<NT>& L, int warp, int lane,
+                                           const unsigned char* rows, const unsigned char* scales, int scale_step,
+                                           const unsigned char* query, uint32_t seen, bool first, uint64_t* empty,
+                                           uint64_t* chain_before, uint32_t chain_parity, uint64_t* chain_mine,
+                                           uint64_t* prob_empty, uint32_t prob_parity) {
+    const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes(), groups = a.sh.groups();
+    float* ss = reinterpret_cast<float*>(sm + L.scratch + warp * (L.kScaleBytes + L.kRatioBytes));  // [group][4 g + j]
+    __half* rr = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(ss) + L.kScaleBytes);   // [group][4 g + j]
+    float* stats = reinterpret_cast<float*>(sm + L.stats) + warp * L.kStats;
+    float* chain = reinterpret_cast<float*>(sm + L.chain);
+
+    // scales of position `lane`: a masked position's is zero, one that is no
+    // scale (NaN, infinite, negative, 2^126 and more) NaN
+    const int mine = 4 * (lane & 7) + (lane >> 3);
+    uint32_t scale[kKv4MaxGroups];
+#pragma unroll
+    for (int gr = 0; gr < kKv4MaxGroups; ++gr) {
+        scale[gr] = 0u;
+        if (gr < groups) {
+            const uint32_t b = (uint32_t)*reinterpret_cast<const uint16_t*>(scales + gr * scale_step) << 16;
+            if ((seen >> lane & 1) && b != 0x80000000u) scale[gr] = b >= 0x7e800000u ? 0x7fc00000u : b;
+            ss[gr * kUnit + mine] = __uint_as_float(scale[gr]);
+        }
+    }
+    __syncwarp();
+
+    float S[2][NT][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[i][n][r] = 0.f;
+    const unsigned char* row = rows + g * rb + t * 8;
+    const uint4* qf = reinterpret_cast<const uint4*>(query) + lane;
+    const int blocks = (a.sh.kv_lora + a.sh.rope) / 64;
+    uint2 w[2][2];  // the block at hand: rows 8 (2 i + h) + g, the lane's two words of 64 values
+    auto fetch = [&](int blk) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[i][h] = *reinterpret_cast<const uint2*>(row + 8 * (2 * i + h) * rb + blk * 32);
+    };
+    fetch(0);
+    float D[2][NT][4];
+    // D = or += the products over block `blk`; the next block's words are on their way meanwhile
+    auto products = [&](int blk, bool begins) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+            uint4 b[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) b[n] = qf[((2 * blk + sub) * NT + n) * 32];
+            uint32_t lo[2][4], hi[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                unpack8(sub ? w[i][0].y : w[i][0].x, lo[i]);
+                unpack8(sub ? w[i][1].y : w[i][1].x, hi[i]);
+            }
+            if (sub == 1 && blk + 1 < blocks) fetch(blk + 1);
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t A[4] = {lo[i][2 * st], hi[i][2 * st], lo[i][2 * st + 1], hi[i][2 * st + 1]};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (begins && sub == 0 && st == 0)
+                            mma_f16(D[i][n], A, b[n].x, b[n].y, zero);
+                        else
+                            mma_f16(D[i][n], A, st ? b[n].z : b[n].x, st ? b[n].w : b[n].y, D[i][n]);
+                    }
+                }
+        }
+    };
+    auto scaled = [&](int gr) {
+        const float4 s4 = *reinterpret_cast<const float4*>(ss + gr * kUnit + 4 * g);
+        const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[i][n][r] = fmaf(s[2 * i + (r >> 1)], D[i][n][r], S[i][n][r]);
+    };
+#pragma unroll 1
+    for (int gr = 0; gr < groups - 1; ++gr) {
+        products(2 * gr, true);
+        products(2 * gr + 1, false);
+        scaled(gr);
+    }
+    products(2 * (groups - 1), true);
+    if (a.sh.rope > 64) products(2 * groups - 1, false);
+    scaled(groups - 1);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty);  // codes and scales of this unit are read
+
+    // scores, and the lane's largest of each head
+    const float* factor = reinterpret_cast<const float*>(query + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
+    float top[NT][2], R[NT][2];
+    const uint32_t hidden = ~seen >> g;  // bit 8 j: position 8 j + g is not seen
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float2 f = *reinterpret_cast<const float2*>(factor + 8 * n + 2 * t);
+        top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                S[i][n][r] = hidden & (1u << (8 * (2 * i + (r >> 1)))) ? -INFINITY : S[i][n][r] * (r & 1 ? f.y : f.x);
+                top[n][r & 1] = fmaxf(top[n][r & 1], S[i][n][r]);
+            }
+    }
+
+    // the references, from the unit before (the item's first waits too: the
+    // last item's must have been read)
+    if (chain_before && !warp_wait(chain_before, chain_parity)) return false;
+    bool moved = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const float2 was = first ? make_float2(-INFINITY, -INFINITY) : *reinterpret_cast<const float2*>(chain + 8 * n + 2 * t);
+        R[n][0] = was.x;
+        R[n][1] = was.y;
+        // (a head that has seen nothing yet takes whatever comes)
+        moved |= top[n][0] > was.x + kRaise || top[n][1] > was.y + kRaise;
+    }
+    moved = __any_sync(0xffffffffu, moved);
+    if (moved) {  // some head's largest of the unit is above its reference by more than that
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int off = 4; off < 32; off <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], off));
+                if (top[n][e] > R[n][e] + kRaise) R[n][e] = top[n][e];
+            }
+    }
+    float ref[4];
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr) {
+        ref[gr] = first ? 0.f : chain[8 * NT + gr];
+        if (gr < groups - 1) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, scale[gr] == 0x7fc00000u ? 0u : scale[gr]);
+            if (__uint_as_float(top) > kRaiseScale * ref[gr]) {
+                ref[gr] = __uint_as_float(((top >> 23) + 1) << 23);
+                moved = true;
+            }
+        }
+    }
+    moved |= first;
+    __syncwarp();
+    if (moved && g == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(chain + 8 * n + 2 * t) = make_float2(R[n][0], R[n][1]);
+        if (t == 0) *reinterpret_cast<float4*>(chain + 8 * NT) = make_float4(ref[0], ref[1], ref[2], ref[3]);
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(chain_mine);
+
+    // ratios s / ref of position `lane`
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr)
+        if (gr < groups - 1) {
+            // 1 / ref: a power of two between 2^-126 and 2^127
+            const float inv = ref[gr] > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(ref[gr])) : 0.f;
+            rr[gr * kUnit + mine] = __float2half_rn(scale[gr] == 0x7fc00000u ? 0.f : __uint_as_float(scale[gr]) * inv);
+        }
+
+    __half2 ph[NT][2][2];
+    float l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float base = R[n][e] == -INFINITY ? 0.f : R[n][e];
+            l[n][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float p0 = exp_of(S[i][n][e] - base), p1 = exp_of(S[i][n][2 + e] - base);
+                l[n][e] += p0 + p1;
+                ph[n][e][i] = __floats2half2_rn(p0, p1);
+            }
         }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-        x *= a.scale;
-        const float mn = fmaxf(m, x), w = m == -INFINITY ? 0.f : expf(m - mn), e = expf(x - mn);
-        m = mn;
-        l = l * w + e;
+    for (int off = 4; off < 32; off <<= 1)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = acc[i] * w + e * v[i];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
+    if (!warp_wait(prob_empty, prob_parity)) return false;
+    if (g == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // as the sums' columns have them: head column 2 t + e is column t + 4 e
+                stats[8 * n + t + 4 * e] = R[n][e];
+                stats[8 * NT + 8 * n + t + 4 * e] = l[n][e];
+            }
+        }
+        if (t == 0) {
+            *reinterpret_cast<float4*>(stats + 16 * NT) = make_float4(ref[0], ref[1], ref[2], ref[3]);
+            stats[16 * NT + 4] = moved ? 1.f : 0.f;
+        }
+    }
+    __syncwarp();
+    // per group: p * s / ref; head column 2 t + e is row t + 4 e
+    unsigned char* pb = sm + L.probs + warp * L.kProbBytes;
+#pragma unroll 1
+    for (int gr = 0; gr < groups - 1; ++gr) {
+        const uint2 rv = *reinterpret_cast<const uint2*>(rr + gr * kUnit + 4 * g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const __half2 y0 = __hmul2(ph[n][e][0], *reinterpret_cast<const __half2*>(&rv.x));
+                const __half2 y1 = __hmul2(ph[n][e][1], *reinterpret_cast<const __half2*>(&rv.y));
+                const int r = t + 4 * e;
+                *reinterpret_cast<uint2*>(pb + ((gr * NT + n) * 8 + r) * 64 + 8 * swizzled(g, r)) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&y0), *reinterpret_cast<const uint32_t*>(&y1));
+            }
+    }
+    __syncwarp();
+    return true;
+}
+
+// ---------------------------------------------------------------- sums
+
+// Head column of the block that column r of n tile n is in the second product.
+__device__ __forceinline__ int column_head(int n, int r) { return 8 * n + 2 * (r & 3) + (r >> 2); }
+
+// What a sum warp carries through an item: lane (g, t) holds latents
+// 8 g + (2 b, 2 b + 1) of its 64, of the columns 2 t and 2 t + 1, in units of
+// ref and relative to R.
+template <int NT>
+struct Sum {
+    float O[4][NT][4], R[NT][2], L[NT][2], ref;
+};
+
+//   rows    the unit's codes, from the warp's first latent
+//   pb      its probabilities, the version of the warp's group
+template <int NT>
+__device__ __forceinline__ void sum_unit(const Mla4Args& a, Sum<NT>& s, int group, int lane, const unsigned char* rows,
+                                         const unsigned char* pb, const float* stats) {
+    const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes();
+    if (stats[16 * NT + 4] != 0.f) {  // the references have moved
+        const float ref = stats[16 * NT + group];
+        const float step = ref > 0.f ? s.ref / ref : 0.f;
+        s.ref = ref;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float R = stats[8 * n + 2 * t + e];
+                const float al = s.R[n][e] == -INFINITY ? 0.f : exp_of(s.R[n][e] - R);
+                s.R[n][e] = R;
+                s.L[n][e] *= al;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    s.O[b][n][e] *= al * step;
+                    s.O[b][n][2 + e] *= al * step;
+                }
+            }
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc_s[warp][i * 32 + lane] = acc[i];
-    if (lane == 0) {
-        m_s[warp] = m;
-        l_s[warp] = l;
+    for (int n = 0; n < NT; ++n) {
+        const float2 l = *reinterpret_cast<const float2*>(stats + 8 * NT + 8 * n + 2 * t);
+        s.L[n][0] += l.x;
+        s.L[n][1] += l.y;
+    }
+    // two steps of 16 positions: lane (g, t)'s k slots are the positions 8 j + 4 st + t
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+        uint32_t w[4];
+        uint2 B[NT];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(rows + (size_t)(8 * j + 4 * st + t) * rb + 4 * g);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) B[n] = *reinterpret_cast<const uint2*>(pb + (n * 8 + g) * 64 + 8 * swizzled(4 * st + t, g));
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {  // nibbles 4 part .. 4 part + 3 of two positions side by side
+            uint32_t x[4], y[4];
+            unpack8(__byte_perm(w[0], w[1], part ? 0x7632 : 0x5410), x);
+            unpack8(__byte_perm(w[2], w[3], part ? 0x7632 : 0x5410), y);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // product 2 part + c: nibbles 4 part + 2 c and + 1
+                const uint32_t A[4] = {x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(s.O[2 * part + c][n], A, B[n].x, B[n].y, s.O[2 * part + c][n]);
+            }
+        }
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (kBf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// 8 consecutive latents of one head's output.
+template <bool kBf16>
+__device__ __forceinline__ void put8(const Mla4Args& a, long long at, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2<kBf16>(v[2 * i], v[2 * i + 1]);
+    uint16_t* o = static_cast<uint16_t*>(a.out) + at;
+    if (a.vec)
+        *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+    else
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+}
+
+// The item's result, or this part's share of it into the workspace.
+template <int NT, bool kBf16>
+__device__ __forceinline__ void finish_item(const Mla4Args& a, const Sum<NT>& s, const Walk& w, int part, int lane) {
+    const int g = lane >> 2, t = lane & 3, h0 = w.block * a.block_heads;
+    const bool whole = w.first == 0 && w.end == w.n;
+    const WsLayout ws(a.block_heads, a.sh.kv_lora);
+    const int slot = 2 * blockIdx.x + (w.first == 0 ? 1 : 0), lat = part * 64 + 8 * g;
+    float2* stat = reinterpret_cast<float2*>(a.ws + ws.stats) + (size_t)slot * a.block_heads;
+    float* sums = reinterpret_cast<float*>(a.ws + ws.sums) + (size_t)slot * a.block_heads * a.sh.kv_lora;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int c = column_head(n, 2 * t + e);
+            if (c >= a.block_heads || h0 + c >= a.n_heads) continue;
+            const float L = s.L[n][e], R = s.R[n][e];
+            const float unit = s.ref * (whole && L != 0.f ? 1.f / L : 1.f);
+            float v[8];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                v[2 * b] = s.O[b][n][e] * unit;
+                v[2 * b + 1] = s.O[b][n][2 + e] * unit;
+            }
+            if (whole) {
+                put8<kBf16>(a, (long long)w.row * a.out_row + (long long)(h0 + c) * a.out_head + lat, v);
+            } else {
+                float4* d = reinterpret_cast<float4*>(sums + (size_t)c * a.sh.kv_lora + lat);
+                d[0] = make_float4(v[0], v[1], v[2], v[3]);
+                d[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+            if (part == 0 && g == 0) {
+                if (!whole)
+                    stat[c] = make_float2(R, L);
+                else if (a.lse)
+                    a.lse[(size_t)w.row * a.n_heads + h0 + c] = R == -INFINITY && L == 0.f ? -INFINITY : R + logf(L);
+            }
+        }
+}
+
+// -------------------------------------------------------------- kernel
+
+template <int NT, bool kBf16>
+__global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args a) {
+    extern __shared__ __align__(128) unsigned char sm[];
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], prob_full[kScoreWarps], prob_empty[kScoreWarps],
+        chain[kScoreWarps], query_full[2], query_empty[2];
+    __shared__ uint64_t seen[kMaxStages];  // positions of the stage's tile that the row sees
+    __shared__ long long scan[kAtThreads / 32 + 1];
+    __shared__ int start_item, start_tile;
+    __shared__ long long part_lo, part_hi;  // this CTA's tiles of the list
+    const Smem<NT> L(a.sh, a.stages);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < a.stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kTile / kUnit + kSumWarps);
+        }
+        for (int i = 0; i < kScoreWarps; ++i) {
+            mbar_init(&prob_full[i], 1);
+            mbar_init(&prob_empty[i], kSumWarps);
+            mbar_init(&chain[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&query_full[i], kScoreWarps);
+            mbar_init(&query_empty[i], kScoreWarps);
+        }
+        mbar_init_fence();
+        start_item = start_tile = 0;
+        part_lo = part_hi = 0;
+    }
+    pdl_enter();
+
+    // the tile list's length; a thread counts `per` consecutive rows
+    const int per = (a.n_rows + kAtThreads - 1) / kAtThreads;
+    const int r0 = min(a.n_rows, tid * per), r1 = min(a.n_rows, r0 + per);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) mine += tiles_of(row_length(a, r));
+    long long run = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, run, off);
+        if (lane >= off) run += o;
+    }
+    if (lane == 31) scan[warp] = run;
+    __syncthreads();
+    long long before = run - mine, rows_total = 0;
+    for (int w = 0; w < kAtThreads / 32; ++w) {
+        if (w < warp) before += scan[w];
+        rows_total += scan[w];
+    }
+    // parts in use: never an empty one before a full one
+    const long long total = rows_total * a.blocks;
+    const int parts = total < gridDim.x ? (int)total : (int)gridDim.x;
+    if (tid == 0 && blockIdx.x < parts) {
+        part_lo = total * blockIdx.x / parts;
+        part_hi = total * (blockIdx.x + 1) / parts;
+    }
+    const WsLayout ws(a.block_heads, a.sh.kv_lora);
+    Join* joins = reinterpret_cast<Join*>(a.ws + ws.joins);
+    const bool by_item = a.n_rows * a.blocks <= kMaxCtas;
+    if (tid == 0) {
+        if (!by_item) joins[blockIdx.x] = Join{0, -1, 0};
+        if (blockIdx.x == 0) *reinterpret_cast<unsigned*>(a.ws) = 0u;  // status
     }
     __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < kAtWarps; ++w) M = fmaxf(M, m_s[w]);
-    for (int w = 0; w < kAtWarps; ++w) L += m_s[w] == -INFINITY ? l_s[w] : l_s[w] * expf(m_s[w] - M);
-    for (int i = threadIdx.x; i < a.sh.kv_lora; i += kAtThreads) {
-        float o = 0.f;
-        for (int w = 0; w < kAtWarps; ++w) o += m_s[w] == -INFINITY ? acc_s[w][i] : acc_s[w][i] * expf(m_s[w] - M);
-        if (L != 0.f) o /= L;
-        const long long at = row * a.out_row + h * a.out_head + i;
-        if (type == GLM_CUDA_BF16)
-            static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(o);
-        else
-            static_cast<__half*>(a.out)[at] = __float2half_rn(o);
+    const long long lo = part_lo, hi = part_hi;
+    if (hi > lo) {
+        long long at = before * a.blocks;
+        for (int r = r0; r < r1; ++r) {
+            const long long n = tiles_of(row_length(a, r)), end = at + n * a.blocks;
+            if (lo >= at && lo < end) {
+                start_item = r * a.blocks + (int)((lo - at) / n);
+                start_tile = (int)((lo - at) % n);
+            }
+            // items that begin in this part: whether they go on past it
+            if (by_item) {
+                long long first = at;
+                for (int b = 0; b < a.blocks; ++b, first += n)
+                    if (first >= lo && first < hi)
+                        joins[r * a.blocks + b] = Join{r * a.blocks + b, first + n > hi ? (int)blockIdx.x : -1,
+                                                       (int)(((first + n) * parts - 1) / total)};
+            } else if (hi > at && hi < end && (hi - at) % n != 0) {
+                const long long first = hi - (hi - at) % n;
+                if (first >= lo) joins[blockIdx.x] = Join{r * a.blocks + (int)((hi - at) / n), (int)blockIdx.x,
+                                                          (int)(((first + n) * parts - 1) / total)};
+            }
+            at = end;
+        }
     }
-    if (a.lse && threadIdx.x == 0) a.lse[(size_t)row * a.n_heads + h] = M + logf(L);
+    __syncthreads();
+    Walk w(a, start_item, start_tile, hi - lo);
+    const int stages = a.stages;
+    bool ok = true;
+
+    if (warp >= kProducer) {
+        shrink_registers<kCopyRegs>();
+        if (warp > kProducer) return;
+        // pages a tile spans, and positions of a page that a tile holds
+        const int page = a.sh.page, per_page = page < kTile ? page : kTile, spans = kTile / per_page;
+        const int tiles_per_page = page > kTile ? page / kTile : 1;
+        const int groups = a.sh.groups(), rb = a.sh.row_bytes();
+        const size_t pb = a.sh.page_bytes();
+        int i = 0;
+        Place at;
+        while (ok && w.next()) {
+            const int req = a.row_req[w.row];
+            const int32_t* ids = a.table + (size_t)(w.len > 0 ? req : 0) * a.table_stride;
+            const int n_ids = w.len > 0 ? (int)((w.len + page - 1) / page) : 0;  // table entries of the row
+            // the table is read 32 entries at a time, one batch ahead
+            int base = w.first * spans / tiles_per_page;
+            int now = base + lane < n_ids ? ids[base + lane] : -1;
+            int next = base + 32 + lane < n_ids ? ids[base + 32 + lane] : -1;
+            for (int tile = w.first; tile < w.end; ++tile, ++i, at.forward(1, stages)) {
+                const int stage = at.stage;
+                if (i >= stages && !warp_wait(&empty[stage], at.phase ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                const int entry = page > kTile ? tile / tiles_per_page : tile * spans;
+                if (entry - base >= 32) {
+                    base += 32;
+                    now = next;
+                    next = base + 32 + lane < n_ids ? ids[base + 32 + lane] : -1;
+                }
+                // a tile's entries are in one batch: spans divides 32 and batches start at a tile's first entry
+                const int id = __shfl_sync(0xffffffffu, now, (entry - base + (lane < spans ? lane : 0)) & 31);
+                const bool held = lane < spans && id >= 0 && id < a.n_pages;
+                const unsigned there = __ballot_sync(0xffffffffu, held);
+                uint64_t bits = 0;
+                for (int s = 0; s < spans; ++s)
+                    if (there >> s & 1) bits |= (per_page == 64 ? ~0ull : (1ull << per_page) - 1) << (s * per_page);
+                const long long rest = w.len - (long long)tile * kTile;
+                if (rest < kTile) bits &= rest > 0 ? (1ull << rest) - 1 : 0ull;
+                unsigned char* d = sm + L.ring + stage * L.stage;
+                const uint32_t code_bytes = (uint32_t)(per_page * rb), scale_bytes = (uint32_t)(per_page * 2);
+                if (lane == 0) {
+                    seen[stage] = bits;
+                    mbar_arrive_expect_tx(&full[stage], (uint32_t)__popc(there) * (code_bytes + groups * scale_bytes));
+                }
+                __syncwarp();
+                const int src = __shfl_sync(0xffffffffu, id, 0);
+                if (page <= kTile) {  // a page's codes and all its scales, each one copy
+                    if (held) {
+                        const unsigned char* p = a.pages + (size_t)id * pb;
+                        bulk_copy_g2s(d + lane * code_bytes, p, code_bytes, &full[stage]);
+                        bulk_copy_g2s(d + kTile * rb + lane * groups * scale_bytes, p + (size_t)page * rb,
+                                      groups * scale_bytes, &full[stage]);
+                    }
+                } else if (there) {   // a part of a page: its scales lie in one run per group
+                    const unsigned char* p = a.pages + (size_t)src * pb;
+                    const int off = (tile % tiles_per_page) * kTile;
+                    if (lane == 0) bulk_copy_g2s(d, p + (size_t)off * rb, code_bytes, &full[stage]);
+                    if (lane < groups)
+                        bulk_copy_g2s(d + kTile * rb + lane * scale_bytes, p + (size_t)page * rb + 2 * ((size_t)lane * page + off),
+                                      scale_bytes, &full[stage]);
+                }
+            }
+        }
+        if (!ok)  // let the copies in flight land before leaving
+            for (int j = max(0, i - stages); j < i; ++j) mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
+    } else if (warp < kScoreWarps) {
+        grow_registers<kMathRegs>();
+        const int per = a.sh.page < kTile ? a.sh.page : kTile, per_log = 31 - __clz(per);  // positions of a page in a tile
+        const int rb = a.sh.row_bytes(), groups = a.sh.groups();
+        constexpr int kUnits = kTile / kUnit;
+        unsigned u = 0;  // the next unit
+        // this warp's next unit, and where its tile is
+        unsigned mine = warp;
+        Place at;
+        at.forward(warp / kUnits, stages);
+        // Two queries' room: a warp loads its share of the next item's once it
+        // has done a unit of this one, when the others are through with the
+        // item before. Nobody waits for all at an item's end.
+        bool more = w.next();
+        if (more) {
+            load_query<NT, kBf16>(a, w.row, w.block, sm + L.qf, warp, lane);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&query_full[0]);
+        }
+        for (unsigned item = 0; more && ok; ++item) {
+            unsigned char* query = sm + L.qf + (item & 1) * L.query;
+            const unsigned u0 = u;
+            u += (unsigned)(w.end - w.first) * kUnits;
+            ok = warp_wait(&query_full[item & 1], item >> 1 & 1);
+            bool loaded = false;
+            more = w.next();  // from here on w is the next item
+            for (; ok; mine += kScoreWarps, at.forward(kScoreWarps / kUnits, stages)) {
+                const bool unit = mine < u;
+                if (unit) {
+                    const int p0 = mine % kUnits * kUnit;
+                    ok = warp_wait(&full[at.stage], at.phase);
+                    if (!ok) break;
+                    const unsigned char* tile = sm + L.ring + at.stage * L.stage;
+                    // this lane's position: its scales lie `per` apart from group to group
+                    const unsigned pos = p0 + lane;
+                    const unsigned char* scales = tile + kTile * rb + 2 * ((pos >> per_log) * groups * per + (pos & (per - 1)));
+                    ok = score_unit<NT>(a, sm, L, warp, lane, tile + p0 * rb, scales, 2 * per, query,
+                                        (uint32_t)(seen[at.stage] >> p0), mine == u0, &empty[at.stage],
+                                        mine ? &chain[(mine - 1) % kScoreWarps] : nullptr, (mine - 1) / kScoreWarps & 1,
+                                        &chain[warp], &prob_empty[warp], (mine / kScoreWarps & 1) ^ 1);
+                    if (ok && lane == 0) mbar_arrive(&prob_full[warp]);
+                    if (!ok) break;
+                }
+                if (!loaded && more) {
+                    loaded = true;
+                    const unsigned to = item + 1;
+                    if (to >= 2) ok = warp_wait(&query_empty[to & 1], (to >> 1 & 1) ^ 1);
+                    if (!ok) break;
+                    load_query<NT, kBf16>(a, w.row, w.block, sm + L.qf + (to & 1) * L.query, warp, lane);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&query_full[to & 1]);
+                }
+                if (!unit) break;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&query_empty[item & 1]);
+        }
+    } else {
+        grow_registers<kMathRegs>();
+        const int part = warp - kScoreWarps, group = part / 2;
+        const bool works = part * 64 < a.sh.kv_lora;
+        const int rb = a.sh.row_bytes();
+        unsigned u = 0;
+        Place at;
+        while (ok && w.next()) {
+            Sum<NT> s;
+            s.ref = 0.f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s.R[n][e] = -INFINITY;
+                    s.L[n][e] = 0.f;
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s.O[b][n][r] = 0.f;
+            }
+            for (int tile = w.first; tile < w.end && ok; ++tile, at.forward(1, stages)) {
+                ok = warp_wait(&full[at.stage], at.phase);
+                const unsigned char* rows = sm + L.ring + at.stage * L.stage + part * 32;
+#pragma unroll 1
+                for (int p0 = 0; p0 < kTile && ok; p0 += kUnit, ++u) {
+                    const unsigned buf = u % kScoreWarps;
+                    ok = warp_wait(&prob_full[buf], u / kScoreWarps & 1);
+                    if (ok && works)
+                        sum_unit<NT>(a, s, group, lane, rows + p0 * rb, sm + L.probs + buf * L.kProbBytes + group * NT * 512,
+                                     reinterpret_cast<const float*>(sm + L.stats) + buf * L.kStats);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&prob_empty[buf]);
+                }
+                if (lane == 0) mbar_arrive(&empty[at.stage]);
+            }
+            if (ok && works) finish_item<NT, kBf16>(a, s, w, part, lane);
+        }
+    }
+    if (!ok && lane == 0) atomicExch(reinterpret_cast<unsigned*>(a.ws), 1u);
+}
+
+// ---------------------------------------------------------------- join
+
+// An item that lies in several CTAs' parts. Grid (items or CTAs, whichever are
+// fewer, y). A CTA's four groups of 128 threads, four latents to a
+// thread, take `at_once` different heads, and with at_once = 1 a quarter of
+// the parts each of one.
+constexpr int kJoinGroup = 128, kJoinGroups = 4;
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kJoinGroup* kJoinGroups) mla4_join_kernel(Mla4Args a, int at_once) {
+    __shared__ float4 part_sum[kJoinGroups][kJoinGroup];
+    pdl_enter();
+    const WsLayout ws(a.block_heads, a.sh.kv_lora);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const Join join = reinterpret_cast<const Join*>(a.ws + ws.joins)[blockIdx.x];
+    if (*reinterpret_cast<const volatile unsigned*>(a.ws) != 0u) {
+        // a wait gave up: no result is to be taken for one
+        const long long n = (long long)a.n_rows * a.n_heads * a.sh.kv_lora;
+        const long long all = (long long)gridDim.x * gridDim.y * blockDim.x;
+        for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + tid; i < n; i += all) {
+            const long long rh = i / a.sh.kv_lora;
+            const long long at = rh / a.n_heads * a.out_row + rh % a.n_heads * a.out_head + i % a.sh.kv_lora;
+            static_cast<uint16_t*>(a.out)[at] = 0x7fff;  // NaN in either type
+            if (a.lse && i % a.sh.kv_lora == 0) a.lse[rh] = __uint_as_float(0x7fc00000u);
+        }
+        return;
+    }
+    if (join.first < 0) return;
+    const int row = join.item / a.blocks, block = join.item - row * a.blocks, p0 = join.first, parts = join.last - p0 + 1;
+    const int heads = min(a.block_heads, a.n_heads - block * a.block_heads);
+    const int group = tid / kJoinGroup, at = tid % kJoinGroup, sharing = kJoinGroups / at_once;
+    const bool latents = 4 * at < a.sh.kv_lora;
+    // part k's share: the second of the CTA it begins in, the first of the others
+    auto slot = [&](int k) { return (size_t)(2 * (p0 + k) + (k == 0 ? 1 : 0)) * a.block_heads; };
+    for (int c0 = blockIdx.y * at_once; c0 < heads; c0 += gridDim.y * at_once) {
+        const int c = c0 + group % at_once;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float M = -INFINITY, l = 0.f;
+        if (c < heads) {
+            const float2* stats = reinterpret_cast<const float2*>(a.ws + ws.stats) + c;
+            const float* sums = reinterpret_cast<const float*>(a.ws + ws.sums) + (size_t)c * a.sh.kv_lora + 4 * at;
+            for (int k = lane; k < parts; k += 32) M = fmaxf(M, stats[slot(k)].x);  // every warp for itself
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+            const float base = M == -INFINITY ? 0.f : M;
+            for (int k = lane; k < parts; k += 32) {
+                const float2 st = stats[slot(k)];
+                l += exp_of(st.x - base) * st.y;
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+            if (latents) {
+#pragma unroll 8
+                for (int k = group / at_once; k < parts; k += sharing) {
+                    const float4 v = *reinterpret_cast<const float4*>(sums + slot(k) * a.sh.kv_lora);
+                    const float wk = exp_of(stats[slot(k)].x - base);
+                    o.x += wk * v.x;
+                    o.y += wk * v.y;
+                    o.z += wk * v.z;
+                    o.w += wk * v.w;
+                }
+            }
+        }
+        if (sharing > 1) {
+            part_sum[group][at] = o;
+            __syncthreads();
+            if (group < at_once)
+                for (int i = group + at_once; i < kJoinGroups; i += at_once) {
+                    const float4 v = part_sum[i][at];
+                    o.x += v.x;
+                    o.y += v.y;
+                    o.z += v.z;
+                    o.w += v.w;
+                }
+            __syncthreads();
+        }
+        if (group >= at_once || c >= heads) continue;
+        const int h = block * a.block_heads + c;
+        if (latents) {
+            const float inv = l != 0.f ? 1.f / l : 1.f;
+            const uint32_t lo = pack2<kBf16>(o.x * inv, o.y * inv), hi = pack2<kBf16>(o.z * inv, o.w * inv);
+            uint16_t* d = static_cast<uint16_t*>(a.out) + (long long)row * a.out_row + (long long)h * a.out_head + 4 * at;
+            if (a.vec) {
+                *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+            } else {
+                d[0] = (uint16_t)lo;
+                d[1] = (uint16_t)(lo >> 16);
+                d[2] = (uint16_t)hi;
+                d[3] = (uint16_t)(hi >> 16);
+            }
+        }
+        if (a.lse && at == 0) a.lse[(size_t)row * a.n_heads + h] = M == -INFINITY && l == 0.f ? -INFINITY : M + logf(l);
+    }
+}
+
+template <int NT, bool kBf16>
+cudaError_t launch_attention(Mla4Args a, int ctas, cudaStream_t st) {
+    constexpr int kMost = 225 * 1024;
+    a.stages = kMaxStages;
+    while (a.stages > 2 && Smem<NT>(a.sh, a.stages).bytes > kMost) --a.stages;
+    const int smem = Smem<NT>(a.sh, a.stages).bytes;
+    auto kernel = mla4_attention_kernel<NT, kBf16>;
+    if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem)) return e;
+    if (cudaError_t e = launch_pdl(kernel, ctas, kAtThreads, (size_t)smem, st, a)) return e;
+    auto join = mla4_join_kernel<kBf16>;
+    // many items: a few parts each, and four heads to a CTA; few items: many
+    // parts each, and a CTA to a head
+    const long long items = (long long)a.n_rows * a.blocks;
+    const int at_once = items >= ctas / 8 ? kJoinGroups : 1;
+    const unsigned lists = (unsigned)(items <= kMaxCtas ? items : ctas);
+    return launch_pdl(join, dim3(lists, (a.block_heads + at_once - 1) / at_once), kJoinGroups * kJoinGroup, 0, st, a, at_once);
 }
 
 }  // namespace
@@ -114,7 +1078,7 @@ __global__ void __launch_bounds__(kAtThreads) mla4_attention_kernel(Mla4Args a, 
 
 extern "C" size_t glm_cuda_mla4_workspace_bytes(int n_rows, int n_heads, int kv_lora_rank) {
     if (n_rows < 1 || n_heads < 1 || kv_lora_rank < 1) return 0;
-    return 16;
+    return glmq::WsLayout(glmq::heads_per_block(n_heads), kv_lora_rank).bytes;
 }
 
 extern "C" int glm_cuda_mla4_attention_async(const GlmCudaKv4Cache* cache, const void* q_dev, int type,
@@ -137,13 +1101,48 @@ extern "C" int glm_cuda_mla4_attention_async(const GlmCudaKv4Cache* cache, const
     if (ws_bytes < glm_cuda_mla4_workspace_bytes(n_rows, n_heads, cache->kv_lora_rank))
         return op_fail(GLM_CUDA_ERR_ARG, fn, "workspace of %zu bytes (need %zu)", ws_bytes,
                        glm_cuda_mla4_workspace_bytes(n_rows, n_heads, cache->kv_lora_rank));
-    Mla4Args a{Kv4Shape{cache->kv_lora_rank, cache->rope_dim, cache->page_size},
-               static_cast<const unsigned char*>(cache->pages), cache->n_pages, q_dev, q_row_stride, q_head_stride,
-               block_table_dev, table_stride, n_req, row_req_dev, row_pos_dev, n_heads, scale, out_dev,
-               out_row_stride, out_head_stride, lse_dev};
-    cudaError_t e = launch_pdl(mla4_attention_kernel, dim3(n_rows, n_heads), kAtThreads, 0,
-                               static_cast<cudaStream_t>(stream), a, type);
-    if (e) return launch_failed(fn, e);
-    count_launches(1);
+    int sms = 0;
+    if (cudaError_t e = current_sms(&sms)) return launch_failed(fn, e);
+    const int ctas = sms < kMaxCtas ? sms : kMaxCtas;
+    if (ctas < 2) return op_fail(GLM_CUDA_ERR_CUDA, fn, "%d SMs", sms);
+    Mla4Args a{};
+    a.sh = Kv4Shape{cache->kv_lora_rank, cache->rope_dim, cache->page_size};
+    a.pages = static_cast<const unsigned char*>(cache->pages);
+    a.n_pages = cache->n_pages;
+    a.q = q_dev;
+    a.q_row = q_row_stride;
+    a.q_head = q_head_stride;
+    a.table = block_table_dev;
+    a.table_stride = table_stride;
+    a.n_req = n_req;
+    a.row_req = row_req_dev;
+    a.row_pos = row_pos_dev;
+    a.n_rows = n_rows;
+    a.n_heads = n_heads;
+    a.blocks = head_blocks(n_heads);
+    a.block_heads = heads_per_block(n_heads);
+    a.scale = scale;
+    a.out = out_dev;
+    a.out_row = out_row_stride;
+    a.out_head = out_head_stride;
+    a.lse = lse_dev;
+    a.ws = static_cast<unsigned char*>(ws_dev);
+    // 16-byte accesses to q and out where all their rows allow them, single values elsewhere
+    a.vec = aligned(q_dev, 16) && aligned(out_dev, 16) && q_row_stride % 8 == 0 && q_head_stride % 8 == 0 &&
+            out_row_stride % 8 == 0 && out_head_stride % 8 == 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    try {
+        // n tiles of 8 heads
+        const int nt = (a.block_heads + 7) / 8;
+        cudaError_t e;
+        if (type == GLM_CUDA_BF16)
+            e = nt == 1 ? launch_attention<1, true>(a, ctas, st) : nt == 2 ? launch_attention<2, true>(a, ctas, st) : launch_attention<3, true>(a, ctas, st);
+        else
+            e = nt == 1 ? launch_attention<1, false>(a, ctas, st) : nt == 2 ? launch_attention<2, false>(a, ctas, st) : launch_attention<3, false>(a, ctas, st);
+        if (e) return launch_failed(fn, e);
+        count_launches(2);
+    } catch (...) {
+        return op_fail(GLM_CUDA_ERR_NOMEM, fn, "host allocation failed");
+    }
     return 0;
 }
