@@ -16,9 +16,9 @@
 // data a group of 128 costs 1.9 dB of signal to noise against one of 32 (19.7
 // against 21.6 dB) and 7.5 % fewer bytes.
 //
-// Why the code is v + 8: a byte b in 0..15 read as an e4m3 number is exactly
-// b * 2^-9 (0..7 are its subnormals, 8..15 its first binade), so the two
-// halves of a byte are tensor-core operands after one AND.
+// Why the code is v + 8: put into the low mantissa bits of the f16 number 1024
+// it is 1024 + v + 8 exactly, so that one packed subtraction turns two codes
+// into tensor-core operands, without a sign to extend.
 #pragma once
 
 #include <cstddef>

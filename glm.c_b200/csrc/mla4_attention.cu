@@ -21,20 +21,14 @@
 // words in shared memory straight into fragments: four bits put into the
 // mantissa of 1024 are 1024 + u (or 1024 + 16 u), and one packed operation
 // makes it v = u - 8, exactly, two values at a time. The query is exact in f16
-// after a power of two per head; the probabilities are rounded to f16 (11
-// bits, relative to the tile's largest).
-// At 20 heads a position takes 12.75 of these instructions, 25.5 clocks of an
-// SM at the measured 0.50 a clock, against 13.3 clocks for its 298 bytes from
-// memory: the tensor pipe is the bound. Measured on the way here: the e4m3
-// form of the instruction is no faster (it is unpacked to f16 first, 3.6 times
-// the instructions); int8 does twice the products a clock but needs two digits
-// for either operand. tcgen05 would need the cached operand written to shared
-// memory as bytes and read back for each product, by count 17 to 22 clocks a
-// position of shared-memory traffic.
+// after a power of two per head. The probabilities are rounded to f16 (11
+// bits): p is held relative to a reference within e^4 of its running maximum,
+// and once more when a scale is multiplied in: 2^-12 of the position's own
+// weight each time, which is below the output's rounding.
 //
 // Scales. A position has one scale per 128 latents. The first product ends at
-// each group and is multiplied into the score; for the second the scale goes
-// into the probability, in one version per group: p * s / ref_g.
+// each group and is multiplied into the score; for the second a group's sum
+// warps multiply it into the probabilities' fragments: p * s / ref_g.
 //
 // References. p = e^(x - R) with R the item's running reference per head, not
 // its maximum: R moves up to a unit's maximum when that exceeds it by more
@@ -47,7 +41,22 @@
 // Roles. Warp 16 copies tiles of 64 positions into a ring in shared memory
 // (cp.async.bulk, completion on mbarriers). Warps 0-7 take a unit of 32
 // positions each in turn: scores, references, the probabilities in f16. Warps
-// 8-15 own 64 latents each: the second product of every unit.
+// 8-15 own 64 latents each: the second product of every tile. The two kinds
+// split the registers (112 a thread) and run on different tiles, so one's
+// products cover the other's unpacking and exponentials.
+//
+// What bounds it, measured at 16 requests of 32768 positions, 20 heads of 512 +
+// 64 (153 MB of cache): 132 us, 1.16 TB/s. The products take 43 % of the tensor
+// pipe's time, the instructions around them (unpacking, scales, waits) keep 53 %
+// of the issue slots; 16 warps of 112 registers are all that an SM holds, too
+// few to fill the rest. At one request of 1500 positions it takes 21 us, most
+// of it three dependent steps: the query's load, one tile a CTA, the join.
+// Tried on the way here and slower at that size: 12 score and 4 sum warps (200
+// us: spills), the sum warps in units of 32 positions (137 us: a wait for each),
+// tcgen05 with the codes spread to bytes in shared memory (192 us: the warps
+// that spread the codes and read the accumulators back are the bound).
+// m16n8k32 e4m3, for which the codes need no arithmetic, issues at 0.21 a clock
+// of an SM against 0.50 for f16: no faster.
 
 #include <cfloat>
 #include <climits>
@@ -125,8 +134,9 @@ __host__ __device__ inline int heads_per_block(int n_heads) {
 
 template <int NT>
 struct Smem {
-    static constexpr int kScaleBytes = kKv4MaxGroups * kUnit * 4, kRatioBytes = 4 * kUnit * 2;
-    static constexpr int kProbBytes = 4 * NT * 8 * kUnit * 2;  // [group][n tile][8 heads][32 positions]
+    static constexpr int kScaleBytes = kKv4MaxGroups * kUnit * 4;
+    static constexpr int kRatios = NT * 8 * kUnit * 2;          // after the probabilities [n tile][8 heads][32 positions]:
+    static constexpr int kProbBytes = kRatios + 4 * kUnit * 2;  // s / ref [group][32 positions], f16 both
     static constexpr int kStats = 16 * NT + 8;                 // R [8 NT], l [8 NT], ref [4], moved, pad
     int qf, query, scratch, probs, stats, chain, ring, stage, bytes;
     __host__ __device__ Smem(const Kv4Shape& sh, int stages) {
@@ -135,8 +145,8 @@ struct Smem {
         qf = o;      // two items' queries: [word][n tile][lane] 16 bytes, the fragments of the word's two steps, ...
         query = words * NT * 512 + 8 * NT * 4;  // ... then each column's factor [8 NT]
         o += 2 * query;
-        scratch = o; // per score warp: scales, ratios
-        o += kScoreWarps * (kScaleBytes + kRatioBytes);
+        scratch = o; // per score warp: scales
+        o += kScoreWarps * kScaleBytes;
         probs = o;   // per score warp
         o += kScoreWarps * kProbBytes;
         stats = o;   // per score warp
@@ -190,9 +200,9 @@ __device__ __forceinline__ float exp_of(float d) {
 
 // Registers of the calling warpgroup's threads. The launch has 96 for each of
 // 640 threads, 5 x 96 = 480 over a thread of every group; the groups' shares
-// are 32 + 4 x 112.
-constexpr int kCopyRegs = 32, kMathRegs = 112;
-static_assert(kCopyRegs + 4 * kMathRegs <= 5 * 96, "more registers than the launch has");
+// are 32 + 2 x 112 + 2 x 112.
+constexpr int kCopyRegs = 32, kScoreRegs = 112, kSumRegs = 112;
+static_assert(kCopyRegs + 2 * kScoreRegs + 2 * kSumRegs <= 5 * 96, "more registers than the launch has");
 template <int kRegs>
 __device__ __forceinline__ void shrink_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegs));
@@ -263,7 +273,7 @@ __device__ __forceinline__ void load_query(const Mla4Args& a, int row, int block
     const int h0 = block * a.block_heads;
     float* factor = reinterpret_cast<float*>(qf + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
     // warp w has the heads w, w + 8, ...: all their loads go out before the first is used
-    static_assert(kScoreWarps == 8, "a head of each n tile to a warp");
+    if (warp >= 8) return;
     uint32_t raw[NT][3][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -348,8 +358,7 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
                                            uint64_t* chain_before, uint32_t chain_parity, uint64_t* chain_mine,
                                            uint64_t* prob_empty, uint32_t prob_parity) {
     const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes(), groups = a.sh.groups();
-    float* ss = reinterpret_cast<float*>(sm + L.scratch + warp * (L.kScaleBytes + L.kRatioBytes));  // [group][4 g + j]
-    __half* rr = reinterpret_cast<__half*>(reinterpret_cast<unsigned char*>(ss) + L.kScaleBytes);   // [group][4 g + j]
+    float* ss = reinterpret_cast<float*>(sm + L.scratch + warp * L.kScaleBytes);  // [group][4 g + j]
     float* stats = reinterpret_cast<float*>(sm + L.stats) + warp * L.kStats;
     float* chain = reinterpret_cast<float*>(sm + L.chain);
 
@@ -394,18 +403,15 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
             uint4 b[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) b[n] = qf[((2 * blk + sub) * NT + n) * 32];
-            uint32_t lo[2][4], hi[2][4];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                unpack8(sub ? w[i][0].y : w[i][0].x, lo[i]);
-                unpack8(sub ? w[i][1].y : w[i][1].x, hi[i]);
-            }
-            if (sub == 1 && blk + 1 < blocks) fetch(blk + 1);
+                uint32_t lo[4], hi[4];
+                unpack8(sub ? w[i][0].y : w[i][0].x, lo);
+                unpack8(sub ? w[i][1].y : w[i][1].x, hi);
+                if (sub == 1 && i == 1 && blk + 1 < blocks) fetch(blk + 1);
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t A[4] = {lo[i][2 * st], hi[i][2 * st], lo[i][2 * st + 1], hi[i][2 * st + 1]};
+                for (int st = 0; st < 2; ++st) {
+                    const uint32_t A[4] = {lo[2 * st], hi[2 * st], lo[2 * st + 1], hi[2 * st + 1]};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
@@ -415,6 +421,7 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
                             mma_f16(D[i][n], A, st ? b[n].z : b[n].x, st ? b[n].w : b[n].y, D[i][n]);
                     }
                 }
+            }
         }
     };
     auto scaled = [&](int gr) {
@@ -501,15 +508,6 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
     __syncwarp();
     if (lane == 0) mbar_arrive(chain_mine);
 
-    // ratios s / ref of position `lane`
-#pragma unroll
-    for (int gr = 0; gr < 4; ++gr)
-        if (gr < groups - 1) {
-            // 1 / ref: a power of two between 2^-126 and 2^127
-            const float inv = ref[gr] > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(ref[gr])) : 0.f;
-            rr[gr * kUnit + mine] = __float2half_rn(scale[gr] == 0x7fc00000u ? 0.f : __uint_as_float(scale[gr]) * inv);
-        }
-
     __half2 ph[NT][2][2];
     float l[NT][2];
 #pragma unroll
@@ -546,23 +544,24 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
             stats[16 * NT + 4] = moved ? 1.f : 0.f;
         }
     }
-    __syncwarp();
-    // per group: p * s / ref; head column 2 t + e is row t + 4 e
+    // head column 2 t + e is row t + 4 e; and the ratios s / ref of position `lane`
     unsigned char* pb = sm + L.probs + warp * L.kProbBytes;
-#pragma unroll 1
-    for (int gr = 0; gr < groups - 1; ++gr) {
-        const uint2 rv = *reinterpret_cast<const uint2*>(rr + gr * kUnit + 4 * g);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const __half2 y0 = __hmul2(ph[n][e][0], *reinterpret_cast<const __half2*>(&rv.x));
-                const __half2 y1 = __hmul2(ph[n][e][1], *reinterpret_cast<const __half2*>(&rv.y));
-                const int r = t + 4 * e;
-                *reinterpret_cast<uint2*>(pb + ((gr * NT + n) * 8 + r) * 64 + 8 * swizzled(g, r)) =
-                    make_uint2(*reinterpret_cast<const uint32_t*>(&y0), *reinterpret_cast<const uint32_t*>(&y1));
-            }
-    }
+        for (int e = 0; e < 2; ++e) {
+            const int r = t + 4 * e;
+            *reinterpret_cast<uint2*>(pb + (n * 8 + r) * 64 + 8 * swizzled(g, r)) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&ph[n][e][0]), *reinterpret_cast<const uint32_t*>(&ph[n][e][1]));
+        }
+    __half* rr = reinterpret_cast<__half*>(pb + L.kRatios);
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr)
+        if (gr < groups - 1) {
+            // 1 / ref: a power of two between 2^-126 and 2^127
+            const float inv = ref[gr] > 0.f ? __uint_as_float(0x7f000000u - __float_as_uint(ref[gr])) : 0.f;
+            rr[gr * kUnit + mine] = __float2half_rn(scale[gr] == 0x7fc00000u ? 0.f : __uint_as_float(scale[gr]) * inv);
+        }
     __syncwarp();
     return true;
 }
@@ -573,63 +572,91 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
 __device__ __forceinline__ int column_head(int n, int r) { return 8 * n + 2 * (r & 3) + (r >> 2); }
 
 // What a sum warp carries through an item: lane (g, t) holds latents
-// 8 g + (2 b, 2 b + 1) of its 64, of the columns 2 t and 2 t + 1, in units of
-// ref and relative to R.
+// 8 g + (2 b, 2 b + 1) of its 64, of the columns 2 t and 2 t + 1, in
+// units of ref and relative to R.
 template <int NT>
 struct Sum {
     float O[4][NT][4], R[NT][2], L[NT][2], ref;
 };
 
-//   rows    the unit's codes, from the warp's first latent
-//   pb      its probabilities, the version of the warp's group
+// The references a unit was scored with, where they have moved.
 template <int NT>
-__device__ __forceinline__ void sum_unit(const Mla4Args& a, Sum<NT>& s, int group, int lane, const unsigned char* rows,
-                                         const unsigned char* pb, const float* stats) {
+__device__ __forceinline__ void follow(Sum<NT>& s, int group, int t, const float* stats) {
+    if (stats[16 * NT + 4] == 0.f) return;
+    const float ref = stats[16 * NT + group];
+    const float step = ref > 0.f ? s.ref / ref : 0.f;
+    s.ref = ref;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float R = stats[8 * n + 2 * t + e];
+            const float al = s.R[n][e] == -INFINITY ? 0.f : exp_of(s.R[n][e] - R);
+            s.R[n][e] = R;
+            s.L[n][e] *= al;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                s.O[b][n][e] *= al * step;
+                s.O[b][n][2 + e] *= al * step;
+            }
+        }
+}
+
+// A tile's two units, in four steps of 16 positions: of step st lane (g, t)'s k
+// slots are the positions 32 (st / 2) + 8 j + 4 (st & 1) + t. A step's words and
+// fragments are loaded while the one before is multiplied.
+//   rows    the tile's codes, from the warp's first latent
+//   probs   the units' buffers, one after the other; ratios: the group's in the first
+template <int NT>
+__device__ __forceinline__ void sum_tile(const Mla4Args& a, Sum<NT>& s, int group, int lane, const unsigned char* rows,
+                                         const unsigned char* probs, const unsigned char* ratios, const float* stats) {
+    constexpr int kUnits = kTile / kUnit, kSteps = kTile / 16;
     const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes();
-    if (stats[16 * NT + 4] != 0.f) {  // the references have moved
-        const float ref = stats[16 * NT + group];
-        const float step = ref > 0.f ? s.ref / ref : 0.f;
-        s.ref = ref;
+    const unsigned char* p = rows + t * rb + 4 * g;
+    struct Step {
+        uint32_t w[4];
+        uint2 q[NT], r;
+    } at[2];
+    auto fetch = [&](int st, Step& f) {
+        const int unit = st >> 1, half = st & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.w[j] = *reinterpret_cast<const uint32_t*>(p + (32 * unit + 8 * j + 4 * half) * rb);
+        f.r = *reinterpret_cast<const uint2*>(ratios + unit * Smem<NT>::kProbBytes + 8 * (4 * half + t));
 #pragma unroll
         for (int n = 0; n < NT; ++n)
+            f.q[n] = *reinterpret_cast<const uint2*>(probs + unit * Smem<NT>::kProbBytes + (n * 8 + g) * 64 + 8 * swizzled(4 * half + t, g));
+    };
+    fetch(0, at[0]);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float R = stats[8 * n + 2 * t + e];
-                const float al = s.R[n][e] == -INFINITY ? 0.f : exp_of(s.R[n][e] - R);
-                s.R[n][e] = R;
-                s.L[n][e] *= al;
+    for (int st = 0; st < kSteps; ++st) {
+        if (st % (kSteps / kUnits) == 0) {
+            const float* u = stats + st / (kSteps / kUnits) * Smem<NT>::kStats;
+            follow<NT>(s, group, t, u);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    s.O[b][n][e] *= al * step;
-                    s.O[b][n][2 + e] *= al * step;
-                }
+            for (int n = 0; n < NT; ++n) {
+                const float2 l = *reinterpret_cast<const float2*>(u + 8 * NT + 8 * n + 2 * t);
+                s.L[n][0] += l.x;
+                s.L[n][1] += l.y;
             }
-    }
+        }
+        const Step& f = at[st & 1];
+        if (st + 1 < kSteps) fetch(st + 1, at[(st + 1) & 1]);
+        uint32_t B[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const float2 l = *reinterpret_cast<const float2*>(stats + 8 * NT + 8 * n + 2 * t);
-        s.L[n][0] += l.x;
-        s.L[n][1] += l.y;
-    }
-    // two steps of 16 positions: lane (g, t)'s k slots are the positions 8 j + 4 st + t
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-        uint32_t w[4];
-        uint2 B[NT];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(rows + (size_t)(8 * j + 4 * st + t) * rb + 4 * g);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) B[n] = *reinterpret_cast<const uint2*>(pb + (n * 8 + g) * 64 + 8 * swizzled(4 * st + t, g));
+        for (int n = 0; n < NT; ++n) {
+            asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][0]) : "r"(f.q[n].x), "r"(f.r.x));
+            asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][1]) : "r"(f.q[n].y), "r"(f.r.y));
+        }
 #pragma unroll
         for (int part = 0; part < 2; ++part) {  // nibbles 4 part .. 4 part + 3 of two positions side by side
             uint32_t x[4], y[4];
-            unpack8(__byte_perm(w[0], w[1], part ? 0x7632 : 0x5410), x);
-            unpack8(__byte_perm(w[2], w[3], part ? 0x7632 : 0x5410), y);
+            unpack8(__byte_perm(f.w[0], f.w[1], part ? 0x7632 : 0x5410), x);
+            unpack8(__byte_perm(f.w[2], f.w[3], part ? 0x7632 : 0x5410), y);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {  // product 2 part + c: nibbles 4 part + 2 c and + 1
                 const uint32_t A[4] = {x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(s.O[2 * part + c][n], A, B[n].x, B[n].y, s.O[2 * part + c][n]);
+                for (int n = 0; n < NT; ++n) mma_f16(s.O[2 * part + c][n], A, B[n][0], B[n][1], s.O[2 * part + c][n]);
             }
         }
     }
@@ -861,7 +888,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
         if (!ok)  // let the copies in flight land before leaving
             for (int j = max(0, i - stages); j < i; ++j) mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
     } else if (warp < kScoreWarps) {
-        grow_registers<kMathRegs>();
+        grow_registers<kScoreRegs>();
         const int per = a.sh.page < kTile ? a.sh.page : kTile, per_log = 31 - __clz(per);  // positions of a page in a tile
         const int rb = a.sh.row_bytes(), groups = a.sh.groups();
         constexpr int kUnits = kTile / kUnit;
@@ -918,7 +945,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
             if (lane == 0) mbar_arrive(&query_empty[item & 1]);
         }
     } else {
-        grow_registers<kMathRegs>();
+        grow_registers<kSumRegs>();
         const int part = warp - kScoreWarps, group = part / 2;
         const bool works = part * 64 < a.sh.kv_lora;
         const int rb = a.sh.row_bytes();
@@ -939,20 +966,20 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s.O[b][n][r] = 0.f;
             }
-            for (int tile = w.first; tile < w.end && ok; ++tile, at.forward(1, stages)) {
-                ok = warp_wait(&full[at.stage], at.phase);
-                const unsigned char* rows = sm + L.ring + at.stage * L.stage + part * 32;
-#pragma unroll 1
-                for (int p0 = 0; p0 < kTile && ok; p0 += kUnit, ++u) {
-                    const unsigned buf = u % kScoreWarps;
-                    ok = warp_wait(&prob_full[buf], u / kScoreWarps & 1);
-                    if (ok && works)
-                        sum_unit<NT>(a, s, group, lane, rows + p0 * rb, sm + L.probs + buf * L.kProbBytes + group * NT * 512,
-                                     reinterpret_cast<const float*>(sm + L.stats) + buf * L.kStats);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&prob_empty[buf]);
-                }
-                if (lane == 0) mbar_arrive(&empty[at.stage]);
+            for (int tile = w.first; tile < w.end; ++tile, at.forward(1, stages), u += kTile / kUnit) {
+                static_assert(kTile == 2 * kUnit && kScoreWarps % 2 == 0, "a tile's two units lie in neighbouring buffers");
+                const unsigned buf = u % kScoreWarps, parity = u / kScoreWarps & 1;
+                const bool here = mbar_wait_bounded(&full[at.stage], at.phase) && mbar_wait_bounded(&prob_full[buf], parity) &&
+                                  mbar_wait_bounded(&prob_full[buf + 1], parity);
+                ok = __all_sync(0xffffffffu, here);
+                if (!ok) break;
+                const unsigned char* probs = sm + L.probs + buf * L.kProbBytes;
+                if (works)
+                    sum_tile<NT>(a, s, group, lane, sm + L.ring + at.stage * L.stage + part * 32, probs, probs + L.kRatios + group * kUnit * 2,
+                                 reinterpret_cast<const float*>(sm + L.stats) + buf * L.kStats);
+                __syncwarp();
+                if (lane < 2) mbar_arrive(&prob_empty[buf + lane]);
+                if (lane == 2) mbar_arrive(&empty[at.stage]);
             }
             if (ok && works) finish_item<NT, kBf16>(a, s, w, part, lane);
         }

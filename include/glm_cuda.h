@@ -456,9 +456,9 @@ int glm_cuda_kv4_load_async(const GlmCudaKv4Cache *cache, const int64_t *slots_d
  * lse [n_rows][n_heads] (may be NULL) receives ln sum exp(scale * q . k). A
  * position whose page lies outside the pool is not seen; a row that sees
  * nothing (position -1, a request outside [0, n_req)) gives zeros and -inf.
- * Sums and statistics are 32-bit; the probabilities are rounded to 8 bits
- * of significance relative to each 64 positions' largest. 0 <= n_rows <=
- * 16384, 1 <= n_heads <= 256. ws: glm_cuda_mla4_workspace_bytes() bytes,
+ * Sums and statistics are 32-bit; the probabilities, and their products with
+ * the scales, are rounded to f16 (11 bits) relative to the row's largest.
+ * Scales are not negative, as stored. 0 <= n_rows <= 16384, 1 <= n_heads <= 256. ws: glm_cuda_mla4_workspace_bytes() bytes,
  * 16-byte aligned, not shared by calls that may overlap; its contents need
  * no preparation. */
 size_t glm_cuda_mla4_workspace_bytes(int n_rows, int n_heads, int kv_lora_rank);

@@ -4,7 +4,7 @@
 Tolerances, from the number formats:
 * plan, codes, scales, ids: equal.
 * loaded rows: v * s in fp32 is exact (3 + 8 bits), then one rounding to the output's type.
-* attention: the probabilities carry 8 significant bits (2^-9 relative at most, 1.1e-3 rms) and the output one
+* attention: probabilities may be rounded to 8 significant bits (2^-9 relative at most, 1.1e-3 rms), the output has one
   rounding to bf16 (up to 2^-9, 1.7e-3 rms over a binade) or f16 (2^-12): together 2.0e-3 and 1.2e-3 rms, doubled
   here. lse: scores are fp32 sums of at most 640 exact products of the query (bf16: exactly; f16: 12 bits kept
   relative to the head's largest) with the codes, a few 2^-24 of |q| |k| each, and one fp32 sum: 1e-4 absolute.
