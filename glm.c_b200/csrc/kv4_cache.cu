@@ -9,10 +9,12 @@
 // NaN, so that whatever reads it comes out NaN, as a product with that row
 // would; a group whose scale rounds to zero holds zeros.
 //
-// Both are bound by memory traffic. Eight lanes share a group: 16-byte
-// loads (stores) of consecutive lanes touch consecutive addresses, three
-// shuffles give the group's largest magnitude, and a warp has four groups in
-// flight.
+// Both should be bound by memory traffic, and the store is only as long as its
+// arithmetic stays near 10 operations a value: no conversion instruction, no
+// integer division per row, ties decided by one exact quotient for all. Eight
+// lanes share a group, a block has 8 rows: 16-byte loads (stores) of
+// consecutive lanes touch consecutive addresses, three shuffles give a group's
+// largest magnitude, and no load waits for another.
 #include <cstdint>
 
 #include <cuda_bf16.h>
@@ -26,15 +28,17 @@
 namespace glmq {
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr int kGroupLanes = 8;
+constexpr int kBlockRows = 8;
+constexpr int kGroupLanes = 8;  // a block has kBlockRows * groups * kGroupLanes threads: 128 to 320
+constexpr int kMostThreads = kBlockRows * kKv4MaxGroups * kGroupLanes;
+constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: x + kWhole is x rounded to an integer, half to even, in its low bits
 
 struct RowArgs {
     Kv4Shape sh;
     unsigned char* pages;
     long long n_slots;
     const int64_t* slots;
-    long long units;  // rows * groups
+    int rows, page_shift;
     void *latent, *rope;
     long long latent_stride, rope_stride;
 };
@@ -85,141 +89,153 @@ __device__ __forceinline__ void put(T* p, const float (&v)[kN]) {
     }
 }
 
-// rint(x / s) with the quotient rounded to fp32 first, for |x / s| < 8. The
-// product with the rounded reciprocal is within 1.3e-6 of the quotient, so
-// only quotients that close to a half need the division itself.
-__device__ __forceinline__ int code_of(float x, float s, float inv, bool slow) {
-    const float q = x * inv, k = rintf(q);
-    int v = (int)k;
-    if (slow || fabsf(fabsf(q - k) - 0.5f) < 4e-6f) v = (int)rintf(__fdiv_rn(x, s));
-    return min(max(v, -7), 7) + 8;
+// rint(x / s) + 8 in the low four bits, others of which are not zero, for
+// |x / s| < 8, 2^-126 <= s and inv = 1 / s rounded: the quotient's first
+// estimate is within two units of its last place, so the remainder r is exact,
+// and its correction is off by less than 2^-45 of the quotient. That cannot
+// change what q rounds to: x / s with an 8-bit s lies at least 2^-34 of itself
+// from every midpoint of two fp32 numbers, or x would have more than 24 bits.
+__device__ __forceinline__ unsigned code_of(float x, float s, float inv) {
+    const float q0 = x * inv, r = fmaf(-q0, s, x), q = fmaf(r, inv, q0);
+    return __float_as_uint(q + kWhole) + 8u;
 }
 
-// Where unit (row, group) lies: its first value, how many there are, its codes and its scale.
+// The same by the division, for scales below the normal numbers.
+__device__ __noinline__ unsigned code_of_small(float x, float s) {
+    return (unsigned)(min(max((int)rintf(__fdiv_rn(x, s)), -7), 7) + 8);
+}
+
+// Where a thread's unit (row, group) lies: its codes and its scale in the
+// pool, its values in the rows.
 struct Unit {
-    bool ok;
-    int n;
-    const unsigned char* page;
-    size_t codes, scale;
-    size_t latent, rope;  // element offsets of the values (one of them is used)
-    bool is_rope;
+    bool live, is_rope;
+    int n;                // values
+    size_t codes, scale;  // byte offsets of a slot inside the pool
+    size_t first;         // element offset in latent or rope
 };
 
-__device__ __forceinline__ Unit unit_of(const RowArgs& a, long long unit) {
-    const int groups = a.sh.groups();
-    const long long row = unit / groups;
-    const int g = (int)(unit - row * groups);
+__device__ __forceinline__ int unit_row(const RowArgs& a, int& g) {
+    const unsigned u = threadIdx.x / kGroupLanes, row = u / (unsigned)a.sh.groups();
+    g = (int)(u - row * a.sh.groups());
+    return (int)(blockIdx.x * kBlockRows + row);
+}
+
+__device__ __forceinline__ Unit unit_of(const RowArgs& a, int row, int g) {
     Unit u;
-    const long long slot = a.slots[row];
-    u.ok = slot >= 0 && slot < a.n_slots;
-    u.is_rope = g == groups - 1;
+    u.live = row < a.rows;
+    u.is_rope = g == a.sh.groups() - 1;
     u.n = u.is_rope ? a.sh.rope : kKv4Group;
-    const long long page = u.ok ? slot / a.sh.page : 0;
-    const int at = u.ok ? (int)(slot - page * a.sh.page) : 0;
-    u.page = a.pages + (size_t)page * a.sh.page_bytes();
-    u.codes = (size_t)at * a.sh.row_bytes() + (size_t)g * (kKv4Group / 2);
-    u.scale = (size_t)a.sh.page * a.sh.row_bytes() + ((size_t)g * a.sh.page + at) * 2;
-    u.latent = (size_t)row * a.latent_stride + (size_t)g * kKv4Group;
-    u.rope = (size_t)row * a.rope_stride;
+    u.first = u.is_rope ? (size_t)row * a.rope_stride : (size_t)row * a.latent_stride + (size_t)g * kKv4Group;
     return u;
 }
 
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) kv4_store_kernel(RowArgs a) {
-    constexpr int kN = 16 / sizeof(T), kChunks = kKv4Group / (kGroupLanes * kN);  // chunks of a 128-value group
-    pdl_enter();
-    const int l = threadIdx.x % kGroupLanes;
-    const long long per = (long long)gridDim.x * (kRowThreads / kGroupLanes);
-    // every lane of a warp runs the same number of rounds, for the shuffles
-    const long long base = ((long long)blockIdx.x * kRowThreads + (threadIdx.x & ~31)) / kGroupLanes;
-    for (long long u0 = base; u0 < a.units; u0 += per) {
-        const long long unit = u0 + (threadIdx.x & 31) / kGroupLanes;
-        const bool live = unit < a.units;
-        const Unit u = unit_of(a, live ? unit : 0);
-        const T* src = u.is_rope ? static_cast<const T*>(a.rope) + u.rope : static_cast<const T*>(a.latent) + u.latent;
-        float x[kChunks][kN];
-        unsigned top = 0u;  // largest magnitude as bits: NaN lies above infinity
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int e = (c * kGroupLanes + l) * kN;
-#pragma unroll
-            for (int i = 0; i < kN; ++i) x[c][i] = 0.f;
-            if (live && u.ok && e < u.n) get<T, kN, kVec>(src + e, x[c]);
-#pragma unroll
-            for (int i = 0; i < kN; ++i) top = max(top, __float_as_uint(x[c][i]) & 0x7fffffffu);
-        }
-#pragma unroll
-        for (int off = 1; off < kGroupLanes; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
-        if (!live || !u.ok) continue;
-        const bool bad = top >= 0x7f800000u;
-        const __nv_bfloat16 sb = bad ? __ushort_as_bfloat16(0x7fc0) : __float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.f));
-        const float s = __bfloat162float(sb);
-        const bool zero = bad || s == 0.f;
-        const bool slow = s < 1e-37f;  // the reciprocal could overflow
-        const float inv = zero ? 0.f : __frcp_rn(s);
-        unsigned char* page = const_cast<unsigned char*>(u.page);
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int e = (c * kGroupLanes + l) * kN;
-            if (e >= u.n) continue;
-            unsigned w = 0u;
-#pragma unroll
-            for (int i = 0; i < kN; ++i) w |= (unsigned)(zero ? 8 : code_of(x[c][i], s, inv, slow)) << (4 * i);
-            unsigned char* d = page + u.codes + e / 2;
-            if constexpr (kN == 8)
-                *reinterpret_cast<uint32_t*>(d) = w;
-            else
-                *reinterpret_cast<uint16_t*>(d) = (uint16_t)w;
-        }
-        if (l == 0) *reinterpret_cast<__nv_bfloat16*>(page + u.scale) = sb;
-    }
+__device__ __forceinline__ bool place(const RowArgs& a, Unit& u, long long slot, int g) {
+    if (slot < 0 || slot >= a.n_slots) return false;
+    const size_t page = (size_t)(slot >> a.page_shift) * a.sh.page_bytes();
+    const int at = (int)(slot & (a.sh.page - 1));
+    u.codes = page + (size_t)at * a.sh.row_bytes() + (size_t)g * (kKv4Group / 2);
+    u.scale = page + (size_t)a.sh.page * a.sh.row_bytes() + ((size_t)g * a.sh.page + at) * 2;
+    return true;
 }
 
 template <typename T, bool kVec>
-__global__ void __launch_bounds__(kRowThreads) kv4_load_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kMostThreads) kv4_store_kernel(RowArgs a) {
+    constexpr int kN = 16 / sizeof(T), kChunks = kKv4Group / (kGroupLanes * kN);  // chunks of a 128-value group
+    pdl_enter();
+    const int l = threadIdx.x % kGroupLanes;
+    int g;
+    const int row = unit_row(a, g);
+    Unit u = unit_of(a, row, g);
+    const T* src = static_cast<const T*>(u.is_rope ? a.rope : a.latent) + u.first;
+    const long long slot = u.live ? a.slots[row] : -1;
+    float x[kChunks][kN];
+    unsigned top = 0u;  // largest magnitude as bits: NaN lies above infinity
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = (c * kGroupLanes + l) * kN;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) x[c][i] = 0.f;
+        if (u.live && e < u.n) get<T, kN, kVec>(src + e, x[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) top = max(top, __float_as_uint(x[c][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int off = 1; off < kGroupLanes; off <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if (!place(a, u, slot, g)) return;
+    const bool bad = top >= 0x7f800000u;
+    const __nv_bfloat16 sb = bad ? __ushort_as_bfloat16(0x7fc0) : __float2bfloat16_rn(__fdiv_rn(__uint_as_float(top), 7.f));
+    const float s = __bfloat162float(sb);
+    const bool zero = bad || s == 0.f;
+    const bool small = s < 1e-37f;  // its reciprocal could overflow, its quotients be beyond 8
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = (c * kGroupLanes + l) * kN;
+        if (e >= u.n) continue;
+        unsigned w = 0u;
+        if (zero) {
+            w = 0x88888888u;
+        } else if (small) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) w |= code_of_small(x[c][i], s) << (4 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) w += (code_of(x[c][i], s, inv) & 15u) << (4 * i);
+        }
+        unsigned char* d = a.pages + u.codes + e / 2;
+        if constexpr (kN == 8)
+            *reinterpret_cast<uint32_t*>(d) = w;
+        else
+            *reinterpret_cast<uint16_t*>(d) = (uint16_t)w;
+    }
+    if (l == 0) *reinterpret_cast<__nv_bfloat16*>(a.pages + u.scale) = sb;
+}
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(kMostThreads) kv4_load_kernel(RowArgs a) {
     constexpr int kN = 16 / sizeof(T), kChunks = kKv4Group / (kGroupLanes * kN);
     pdl_enter();
     const int l = threadIdx.x % kGroupLanes;
-    const long long per = (long long)gridDim.x * (kRowThreads / kGroupLanes);
-    for (long long unit = ((long long)blockIdx.x * kRowThreads + threadIdx.x) / kGroupLanes; unit < a.units; unit += per) {
-        const Unit u = unit_of(a, unit);
-        T* dst = u.is_rope ? static_cast<T*>(a.rope) + u.rope : static_cast<T*>(a.latent) + u.latent;
-        const float s = u.ok ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(u.page + u.scale)) : 0.f;
-        unsigned w[kChunks];
+    int g;
+    const int row = unit_row(a, g);
+    Unit u = unit_of(a, row, g);
+    if (!u.live) return;
+    T* dst = static_cast<T*>(u.is_rope ? a.rope : a.latent) + u.first;
+    const bool ok = place(a, u, a.slots[row], g);
+    const float s = ok ? __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(a.pages + u.scale)) : 0.f;
+    unsigned w[kChunks];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int e = (c * kGroupLanes + l) * kN;
-            w[c] = 0x88888888u;
-            if (!u.ok || e >= u.n) continue;
-            const unsigned char* p = u.page + u.codes + e / 2;
-            if constexpr (kN == 8)
-                w[c] = *reinterpret_cast<const uint32_t*>(p);
-            else
-                w[c] = *reinterpret_cast<const uint16_t*>(p);
-        }
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = (c * kGroupLanes + l) * kN;
+        w[c] = 0x88888888u;
+        if (!ok || e >= u.n) continue;
+        const unsigned char* p = a.pages + u.codes + e / 2;
+        if constexpr (kN == 8)
+            w[c] = *reinterpret_cast<const uint32_t*>(p);
+        else
+            w[c] = *reinterpret_cast<const uint16_t*>(p);
+    }
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int e = (c * kGroupLanes + l) * kN;
-            if (e >= u.n) continue;
-            float v[kN];
+    for (int c = 0; c < kChunks; ++c) {
+        const int e = (c * kGroupLanes + l) * kN;
+        if (e >= u.n) continue;
+        float v[kN];
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = (float)((int)((w[c] >> (4 * i)) & 15u) - 8) * s;
-            put<T, kN, kVec>(dst + e, v);
-        }
+        for (int i = 0; i < kN; ++i)  // 2^23 + code, exactly
+            v[i] = (__uint_as_float((w[c] >> (4 * i) & 15u) | 0x4b000000u) - 8388616.f) * s;
+        put<T, kN, kVec>(dst + e, v);
     }
 }
 
 enum class Way { kStore, kLoad };
 
 template <typename T>
-cudaError_t launch_rows(Way way, bool vec, const RowArgs& a, int sms, cudaStream_t st) {
-    const long long per = kRowThreads / kGroupLanes;
-    long long grid = (a.units + per - 1) / per;
-    const long long most = (long long)sms * (2048 / kRowThreads);
-    if (grid > most) grid = most;
+cudaError_t launch_rows(Way way, bool vec, const RowArgs& a, cudaStream_t st) {
     auto kernel = way == Way::kStore ? (vec ? kv4_store_kernel<T, true> : kv4_store_kernel<T, false>)
                                      : (vec ? kv4_load_kernel<T, true> : kv4_load_kernel<T, false>);
-    return launch_pdl(kernel, (unsigned)grid, kRowThreads, 0, st, a);
+    return launch_pdl(kernel, (unsigned)((a.rows - 1) / kBlockRows + 1), kBlockRows * kGroupLanes * a.sh.groups(), 0, st, a);
 }
 
 int rows_entry(const char* fn, Way way, const GlmCudaKv4Cache* cache, const int64_t* slots, int n_rows, int type,
@@ -235,14 +251,14 @@ int rows_entry(const char* fn, Way way, const GlmCudaKv4Cache* cache, const int6
     const size_t tb = type_bytes(type);
     if (!aligned(latent, tb) || !aligned(rope, tb) || !aligned(slots, 8))
         return op_fail(GLM_CUDA_ERR_ARG, fn, "a pointer is not aligned to its type");
-    int sms = 0;
-    if (cudaError_t e = current_sms(&sms)) return launch_failed(fn, e);
     RowArgs a;
     a.sh = Kv4Shape{cache->kv_lora_rank, cache->rope_dim, cache->page_size};
     a.pages = static_cast<unsigned char*>(cache->pages);
     a.n_slots = (long long)cache->n_pages * cache->page_size;
     a.slots = slots;
-    a.units = (long long)n_rows * a.sh.groups();
+    a.rows = n_rows;
+    a.page_shift = 0;
+    while (1 << a.page_shift < cache->page_size) ++a.page_shift;
     a.latent = latent;
     a.rope = rope;
     a.latent_stride = latent_stride;
@@ -250,9 +266,9 @@ int rows_entry(const char* fn, Way way, const GlmCudaKv4Cache* cache, const int6
     // 16-byte accesses where every row starts on a 16-byte boundary, one value at a time elsewhere
     const bool vec = aligned(latent, 16) && aligned(rope, 16) && latent_stride * tb % 16 == 0 && rope_stride * tb % 16 == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = type == GLM_CUDA_F32    ? launch_rows<float>(way, vec, a, sms, st)
-                    : type == GLM_CUDA_BF16 ? launch_rows<__nv_bfloat16>(way, vec, a, sms, st)
-                                            : launch_rows<__half>(way, vec, a, sms, st);
+    cudaError_t e = type == GLM_CUDA_F32    ? launch_rows<float>(way, vec, a, st)
+                    : type == GLM_CUDA_BF16 ? launch_rows<__nv_bfloat16>(way, vec, a, st)
+                                            : launch_rows<__half>(way, vec, a, st);
     if (e) return launch_failed(fn, e);
     count_launches(1);
     return 0;
