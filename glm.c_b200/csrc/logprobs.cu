@@ -6,21 +6,26 @@
 //   log p_i = x_i - m - ln l,   entropy = ln l - s / l
 //
 // The logits are read once (620 KB a row for GLM-4.7-Flash's vocabulary in
-// fp32) and that traffic is the bound. Each thread keeps running (m, l, s):
-// raising m by d multiplies l by e^-d and turns s into e^-d (s - d l).
+// fp32), and that traffic is the bound as long as a value costs few
+// instructions. Each thread keeps (m, l, s) relative to a reference that
+// follows its largest value only when that is more than kSlack above, which
+// after the first values it hardly ever is; two values go through one packed
+// fp32 instruction where there is one.
 //
-// The most likely tokens: every warp keeps the best 32 (value, index) pairs
-// it has seen, sorted, one to a lane, as 64-bit keys (ordered value bits, then
-// the complement of the index, so that ties go to the lowest index). A value
-// has to beat the k-th of them to be looked at; those that do collect in a
-// shared-memory buffer and enter 32 at a time by a bitonic sort and merge, so
-// that an ascending row, where every value is a new best, costs a bounded
-// amount per value too. Warps share their bounds: what is below any warp's
-// k-th best is not among the row's.
+// The most likely tokens cost nothing in that pass but each thread's largest
+// value, which it keeps anyway. The k-th largest of a CTA's threads' largest
+// is no larger than the k-th largest value of its part of the row, so what can
+// be among the best lies in the threads whose largest reaches it, k of them
+// unless there are ties. Their values, one in 256 / k, are read again, and
+// those that reach the bound collect in shared memory and enter a warp's
+// sorted list of 32 (one to a lane, as 64-bit keys: ordered value bits, then
+// the complement of the index, so that ties go to the lowest index) 32 at a
+// time by a bitonic sort and merge. No input makes that more than one more
+// reading of the row.
 //
 // A row is one CTA's, or a thread-block cluster's when there are fewer rows
-// than SMs; the CTAs of a cluster meet in distributed shared memory. No
-// workspace, no second launch.
+// than the GPU holds CTAs; the CTAs of a cluster meet in distributed shared
+// memory. No workspace, no second launch.
 #include <cfloat>
 #include <cmath>
 #include <climits>
@@ -38,10 +43,12 @@
 namespace glmq {
 namespace {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 256;
 constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;   // one sorted pair to a lane
 constexpr int kLpMaxCluster = 8;
+constexpr int kLpCtas = 4;      // CTAs an SM holds
+constexpr float kSlack = 8.f;   // a thread's reference may lie this far below its largest value: e^8 in l and s, as floats
 
 struct LpArgs {
     const void* logits;
@@ -53,46 +60,109 @@ struct LpArgs {
     float* top_logprobs;
 };
 
-// Running sums of a part of a row, in units of ln.
+// Running sums of a part of a row; s in units of log2.
 struct Part {
     float m, l, s;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float exp_fast(float d) { return exp2f(d * kLog2e); }
+// 2^t within 2 units of the last place, zero below the normal numbers (nothing beside a sum that holds a one).
+__device__ __forceinline__ float exp2_fast(float t) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(t));
+    return e;
+}
+
+// The part relative to m >= p.m (or, if m is -inf, a part without weight).
+__device__ __forceinline__ Part rebase(const Part& p, float m) {
+    // a part without weight (nothing seen, or all of it -inf) adds nothing
+    const float d = p.m == -INFINITY ? 0.f : (p.m - m) * kLog2e, w = exp2_fast(d);
+    // a weight of zero may stand beside a difference of -inf
+    return Part{m, p.l * w, w > 0.f ? w * (p.s + p.l * d) : w * 0.f};
+}
 
 __device__ __forceinline__ Part join(const Part& a, const Part& b) {
     const float m = fmaxf(a.m, b.m);
-    // a part without weight (nothing seen, or all of it -inf) adds nothing
-    const float da = a.m == -INFINITY ? 0.f : a.m - m, db = b.m == -INFINITY ? 0.f : b.m - m;
-    const float wa = exp_fast(da), wb = exp_fast(db);
-    // a weight of zero may stand beside a difference of -inf
-    const float sa = wa > 0.f ? wa * (a.s + a.l * da) : 0.f, sb = wb > 0.f ? wb * (b.s + b.l * db) : 0.f;
-    return Part{m, a.l * wa + b.l * wb, sa + sb};
+    const Part x = rebase(a, m), y = rebase(b, m);
+    return Part{m, x.l + y.l, x.s + y.s};
 }
 
-// Value and index as one key: larger value first, then the lower index. Zero is below every key.
-__device__ __forceinline__ uint64_t key_of(float x, int i) {
-    const unsigned b = __float_as_uint(x + 0.f);  // -0 ties with +0
-    const unsigned o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return ((uint64_t)o << 32) | (unsigned)~i;
+// Two fp32 values side by side, for the packed instructions.
+struct Two {
+    unsigned long long v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
 }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// A thread's sums: even and odd values apart.
+struct Sums {
+    float m;
+    Two l, s;
+    __device__ __forceinline__ Sums() : m(-INFINITY), l(0.f, 0.f), s(0.f, 0.f) {}
+    __device__ __forceinline__ Part part() const {
+        float a, b, c, d;
+        l.get(a, b);
+        s.get(c, d);
+        return Part{m, a + b, c + d};
+    }
+    // before values up to top are added
+    __device__ __forceinline__ void follow(float top) {
+        if (top <= (m == -INFINITY ? m : m + kSlack)) return;
+        const Part p = rebase(part(), top);
+        m = top;
+        l = Two(p.l, 0.f);
+        s = Two(p.s, 0.f);
+    }
+    __device__ __forceinline__ void add(float x0, float x1) {
+        const float ref = m == -INFINITY ? 0.f : m;
+        const Two t = mul2(add2(Two(x0, x1), Two(-ref, -ref)), Two(kLog2e, kLog2e));
+        float t0, t1;
+        t.get(t0, t1);
+        const Two e(exp2_fast(t0), exp2_fast(t1));
+        l = add2(l, e);
+        s = fma2(e, Two(fmaxf(t0, -300.f), fmaxf(t1, -300.f)), s);  // e is zero there: no 0 * inf
+    }
+};
+
+// Bits in the order of the values; none is zero.
+__device__ __forceinline__ unsigned ordered(float x) {
+    const unsigned b = __float_as_uint(x + 0.f);  // -0 ties with +0
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// Value and index as one key: larger value first, then the lower index. Zero is below every key.
+__device__ __forceinline__ uint64_t key_of(float x, int i) { return ((uint64_t)ordered(x) << 32) | (unsigned)~i; }
 __device__ __forceinline__ float key_value(uint64_t k) {
     const unsigned o = (unsigned)(k >> 32);
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(unsigned)k; }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int off) { return __shfl_xor_sync(0xffffffffu, v, off); }
-
-__device__ __forceinline__ uint64_t keep(uint64_t v, int off, bool larger) {
-    const uint64_t o = shfl_xor64(v, off);
+template <typename K>
+__device__ __forceinline__ K keep(K v, int off, bool larger) {
+    const K o = __shfl_xor_sync(0xffffffffu, v, off);
     return (v > o) == larger ? v : o;
 }
 
 // The warp's 32 keys in descending order.
-__device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
+template <typename K>
+__device__ __forceinline__ K sort32(K v, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -102,19 +172,13 @@ __device__ __forceinline__ uint64_t sort32(uint64_t v, int lane) {
 }
 
 // The 32 largest of two descending lists, in descending order.
-__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-    uint64_t v = a > r ? a : r;
+template <typename K>
+__device__ __forceinline__ K merge32(K a, K b, int lane) {
+    const K r = __shfl_sync(0xffffffffu, b, 31 - lane);
+    K v = a > r ? a : r;
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v = keep(v, off, (lane & off) == 0);
     return v;
-}
-
-// Largest float below x (x itself for -inf).
-__device__ __forceinline__ float below(float x) {
-    if (x == -INFINITY) return x;
-    const int b = __float_as_int(x + 0.f);
-    return b == 0 ? -FLT_MIN * FLT_EPSILON : __int_as_float(b > 0 ? b - 1 : b + 1);
 }
 
 template <typename T>
@@ -134,6 +198,12 @@ struct Vec {
         else
             return __int_as_float(i & 1 ? w[i >> 1] & 0xffff0000 : w[i >> 1] << 16);
     }
+    __device__ __forceinline__ float largest() const {  // NaN aside
+        float t = get(0);
+#pragma unroll
+        for (int i = 1; i < n; ++i) t = fmaxf(t, get(i));
+        return t;
+    }
 };
 
 template <typename T>
@@ -143,170 +213,142 @@ __device__ __forceinline__ float value_of(const T* p, long long i) {
     else return __bfloat162float(p[i]);
 }
 
-// 16-byte loads in flight per thread: 16 values where candidates are
-// collected, so that two CTAs' buffers fit an SM at either width.
-template <typename T, bool kTop>
-constexpr int kLpVecs = kTop ? 16 / Vec<T>::n : 4;
-
-// One warp's candidates: an iteration adds at most 32 lanes x 16 values to
-// fewer than 32 left from before.
-constexpr int kLpBuffer = 32 * 16 + 32;
-
-template <bool kTop>
-constexpr size_t lp_smem() {
-    return kTop ? (size_t)kLpWarps * (kLpBuffer + 32) * 8 : 0;
-}
+constexpr int kLpVecs = 4;                 // 16-byte loads in flight per thread
+constexpr int kLpBuffer = 32 * 8 + 32;     // one warp's candidates: 32 lanes x 8 values to fewer than 32 left from before
 
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LpArgs a, int cluster) {
+__global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(LpArgs a, int cluster) {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
-    constexpr int V = Vec<T>::n, U = kLpVecs<T, kTop>;
-    extern __shared__ __align__(16) uint64_t lp_sm[];
+    constexpr int V = Vec<T>::n, U = kLpVecs;
     __shared__ Part parts[kLpWarps];
     __shared__ Part cta_part;
-    __shared__ int shared_bound;     // ordered bits of the largest bound any warp has published
-    __shared__ int counts[kLpWarps];
+    __shared__ unsigned tops[kTop ? kLpThreads : 1];     // per warp its threads' largest, sorted; then the CTA's 32 largest
+    __shared__ uint64_t lists[kTop ? kLpThreads : 1];    // per warp its best, sorted
+    __shared__ uint64_t buffers[kTop ? kLpWarps * kLpBuffer : 1];
+    __shared__ int counts[kLpWarps], chosen[kLpThreads], n_chosen;
     const int rank = (int)cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long row = blockIdx.x / cluster;
-    uint64_t* lists = lp_sm;                                             // [kLpWarps][32] sorted
-    uint64_t* buffer = lp_sm + kLpWarps * 32 + warp * (kTop ? kLpBuffer : 0);
-    if (kTop && tid < kLpWarps) counts[tid] = 0;
-    if (tid == 0) shared_bound = INT_MIN;
+    if (kTop && lane == 0) counts[warp] = 0;
+    if (tid == 0) n_chosen = 0;
     pdl_enter();
-    __syncthreads();
 
     const T* x = static_cast<const T*>(a.logits) + row * a.stride;
     // the 16-byte vectors of the row; what lies before and after them goes value by value
     const int head = min(a.vocab, (int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)));
-    const int nvec = (a.vocab - head) / V, tail = head + nvec * V;
+    const int nvec = (a.vocab - head) / V, tail = head + nvec * V, edge = head + a.vocab - tail;
     const int v_lo = (int)((long long)rank * nvec / cluster), v_hi = (int)((long long)(rank + 1) * nvec / cluster);
-
-    Part p{-INFINITY, 0.f, 0.f};
-    uint64_t list = 0;          // this lane's entry of the warp's sorted best
-    float bound = -INFINITY;    // a value has to be above it
-
-    // the warp's candidates, 32 at a time, into its list
-    auto take = [&](bool all) {
-        __syncwarp();
-        int n = counts[warp];
-        while (n >= 32 || (all && n > 0)) {
-            const int got = min(n, 32);
-            n -= got;
-            const uint64_t c = lane < got ? buffer[n + lane] : 0;
-            list = merge32(list, sort32(c, lane), lane);
-        }
-        __syncwarp();
-        if (lane == 0) counts[warp] = n;
-        const uint64_t kth = __shfl_sync(0xffffffffu, list, a.top - 1);
-        if (kth) {
-            bound = fmaxf(bound, key_value(kth));
-            if (lane == 0) {
-                const int b = __float_as_int(below(key_value(kth)));
-                atomicMax(&shared_bound, b >= 0 ? b : b ^ 0x7fffffff);  // float order as int order
-            }
-        }
-        __syncwarp();
-    };
-    auto push = [&](float v, int i) {
-        if (v > bound) buffer[atomicAdd(&counts[warp], 1)] = key_of(v, i);
-    };
-    auto add = [&](float v) {
-        if (v > p.m) {
-            const Part q = join(p, Part{v, 0.f, 0.f});
-            p = q;
-        }
-        const float d = v - (p.m == -INFINITY ? 0.f : p.m), e = exp_fast(d);
-        p.l += e;
-        p.s += e * fmaxf(d, -200.f);  // e is zero there: no 0 * inf
-    };
-
-    // values before the first vector: the first warp of the first CTA, before all higher indices
-    if (rank == 0 && warp == 0 && head > 0) {
-        if (lane < head) {
-            const float v = value_of(x, lane);
-            add(v);
-            if constexpr (kTop) push(v, lane);
-        }
-        if constexpr (kTop) take(false);
-    }
     const T* xv = x + head;
-    constexpr int kStep = 32 * U;  // vectors a warp takes at a time, consecutive ones
-    for (int v0 = v_lo + warp * kStep; v0 < v_hi; v0 += kLpWarps * kStep) {
+    // value e of those beside the vectors, fewer than 2 V <= 32: lane e of the first CTA's first warp has it
+    const bool has_edge = rank == 0 && tid < edge;
+    const int edge_index = tid < head ? tid : tail + tid - head;
+
+    Sums sums;
+    float best = -INFINITY;  // of the vectors
+    int v = v_lo + tid;
+    for (; v + (U - 1) * kLpThreads < v_hi; v += U * kLpThreads) {
         Vec<T> r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int v = v0 + u * 32 + lane;
-            if (v < v_hi) r[u].load(xv + (long long)v * V);
-        }
-        float top = -INFINITY;
+        for (int u = 0; u < U; ++u) r[u].load(xv + (long long)(v + u * kLpThreads) * V);
+#pragma unroll
+        for (int u = 0; u < U; ++u) best = fmaxf(best, r[u].largest());
+        sums.follow(best);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (v0 + u * 32 + lane < v_hi)
 #pragma unroll
-                for (int i = 0; i < V; ++i) top = fmaxf(top, r[u].get(i));
-        if (top > p.m) p = join(p, Part{top, 0.f, 0.f});
-        const float m = p.m == -INFINITY ? 0.f : p.m;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (v0 + u * 32 + lane < v_hi)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = r[u].get(i) - m, e = exp_fast(d);
-                    p.l += e;
-                    p.s += e * fmaxf(d, -200.f);
-                }
-        if constexpr (kTop) {
-            const int sb = *reinterpret_cast<volatile int*>(&shared_bound);
-            if (sb != INT_MIN) bound = fmaxf(bound, __int_as_float(sb >= 0 ? sb : sb ^ 0x7fffffff));
-            if (bound == -INFINITY) {
-                // nothing to compare with yet: the k-th largest of the lanes'
-                // own largest values is no larger than the k-th of them all
-                const uint64_t k = sort32(key_of(top, lane), lane);
-                bound = fmaxf(bound, below(key_value(__shfl_sync(0xffffffffu, k, a.top - 1))));
-            }
-            if (__any_sync(0xffffffffu, top > bound)) {
-                if (top > bound) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (v0 + u * 32 + lane < v_hi)
-#pragma unroll
-                            for (int i = 0; i < V; ++i) push(r[u].get(i), head + (v0 + u * 32 + lane) * V + i);
-                }
-                take(false);
-            }
-        }
+            for (int i = 0; i < V; i += 2) sums.add(r[u].get(i), r[u].get(i + 1));
     }
-    // values past the last vector: the last warp of the last CTA
-    if (rank == cluster - 1 && warp == kLpWarps - 1 && tail < a.vocab) {
-        if (tail + lane < a.vocab) {
-            const float v = value_of(x, tail + lane);
-            add(v);
-            if constexpr (kTop) push(v, tail + lane);
-        }
+    for (; v < v_hi; v += kLpThreads) {
+        Vec<T> r;
+        r.load(xv + (long long)v * V);
+        best = fmaxf(best, r.largest());
+        sums.follow(best);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) sums.add(r.get(i), r.get(i + 1));
     }
-
+    float beside = -INFINITY;
+    if (has_edge) {
+        beside = value_of(x, edge_index);
+        sums.follow(fmaxf(best, beside));
+        sums.add(beside, -INFINITY);
+    }
+    Part p = rebase(sums.part(), fmaxf(fmaxf(best, beside), sums.m));
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1)
         p = join(p, Part{__shfl_xor_sync(0xffffffffu, p.m, off), __shfl_xor_sync(0xffffffffu, p.l, off),
                          __shfl_xor_sync(0xffffffffu, p.s, off)});
     if (lane == 0) parts[warp] = p;
+
+    uint64_t list = 0;  // this lane's entry of the warp's sorted best
     if constexpr (kTop) {
+        // the k-th largest of the threads' largest
+        const unsigned mine = best > -INFINITY ? ordered(best) : 0u;
+        unsigned t = sort32(mine, lane);
+        tops[tid] = t;
+        __syncthreads();
+        for (int half = kLpWarps / 2; half > 0; half >>= 1) {
+            if (warp < half) tops[tid] = t = merge32(t, tops[tid + half * 32], lane);
+            __syncthreads();
+        }
+        const unsigned bound = max(tops[a.top - 1], 1u);
+        // who reaches it
+        const unsigned who = __ballot_sync(0xffffffffu, mine >= bound);
+        int at = 0;
+        if (lane == 0 && who) at = atomicAdd(&n_chosen, __popc(who));
+        at = __shfl_sync(0xffffffffu, at, 0);
+        if (mine >= bound) chosen[at + __popc(who & ((1u << lane) - 1u))] = tid;
+        __syncthreads();
+
+        uint64_t* buffer = buffers + warp * kLpBuffer;
+        uint64_t least = (uint64_t)bound << 32;  // a key below it is not among the best
+        // the warp's candidates, 32 at a time, into its list
+        auto take = [&](bool all) {
+            __syncwarp();
+            int n = counts[warp];
+            __syncwarp();
+            if (n < 32 && !all) return;
+            while (n >= 32 || (all && n > 0)) {
+                const int got = min(n, 32);
+                n -= got;
+                const uint64_t c = lane < got ? buffer[n + lane] : 0;
+                list = merge32(list, sort32(c, lane), lane);
+            }
+            __syncwarp();
+            if (lane == 0) counts[warp] = n;
+            const uint64_t kth = __shfl_sync(0xffffffffu, list, a.top - 1);
+            least = max(least, kth);
+            __syncwarp();
+        };
+        auto push = [&](float value, int i) {
+            const uint64_t key = key_of(value, i);
+            if (value > -INFINITY && key >= least) buffer[atomicAdd(&counts[warp], 1)] = key;
+        };
+        if (has_edge) push(beside, edge_index);
+        const int rounds = (v_hi - v_lo + kLpThreads - 1) / kLpThreads;  // vectors of the first thread
+        for (int c = warp; c < n_chosen; c += kLpWarps)
+            for (int q0 = 0; q0 < rounds; q0 += 32) {
+                const int w = v_lo + chosen[c] + (q0 + lane) * kLpThreads;
+                if (q0 + lane < rounds && w < v_hi) {
+                    Vec<T> r;
+                    r.load(xv + (long long)w * V);
+                    if (ordered(r.largest()) >= (unsigned)(least >> 32))
+#pragma unroll
+                        for (int i = 0; i < V; ++i) push(r.get(i), head + w * V + i);
+                }
+                take(false);
+            }
         take(true);
-        lists[warp * 32 + lane] = list;
+        lists[tid] = list;
     }
     __syncthreads();
     if constexpr (kTop) {
         for (int half = kLpWarps / 2; half > 0; half >>= 1) {
-            if (warp < half) {
-                list = merge32(lists[warp * 32 + lane], lists[(warp + half) * 32 + lane], lane);
-                lists[warp * 32 + lane] = list;
-            }
+            if (warp < half) lists[tid] = list = merge32(list, lists[tid + half * 32], lane);
             __syncthreads();
         }
     }
     if (warp == 0) {
-        p = parts[lane % kLpWarps];  // both halves of the warp form the same sum
+        p = parts[lane % kLpWarps];  // every eight lanes of the warp form the same sum
 #pragma unroll
         for (int off = kLpWarps / 2; off > 0; off >>= 1)
             p = join(p, Part{__shfl_xor_sync(0xffffffffu, p.m, off), __shfl_xor_sync(0xffffffffu, p.l, off),
@@ -316,10 +358,20 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LpArgs a, int c
     if (cluster > 1) {
         cl.sync();
         if (rank == 0 && warp == 0) {
-            for (int r = 1; r < cluster; ++r) {
-                p = join(p, *cl.map_shared_rank(&cta_part, r));
-                if constexpr (kTop) list = merge32(list, *cl.map_shared_rank(lists + lane, r), lane);
-            }
+            Part other[kLpMaxCluster];
+            uint64_t keys[kLpMaxCluster];
+#pragma unroll
+            for (int r = 1; r < kLpMaxCluster; ++r)
+                if (r < cluster) {
+                    other[r] = *cl.map_shared_rank(&cta_part, r);
+                    if constexpr (kTop) keys[r] = *cl.map_shared_rank(lists + lane, r);
+                }
+#pragma unroll
+            for (int r = 1; r < kLpMaxCluster; ++r)
+                if (r < cluster) {
+                    p = join(p, other[r]);
+                    if constexpr (kTop) list = merge32(list, keys[r], lane);
+                }
         }
         cl.sync();  // no CTA leaves while its memory may still be read
     }
@@ -328,7 +380,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LpArgs a, int c
     if (lane == 0) {
         // a row with nothing but -inf has no distribution: probability zero, no entropy
         const bool empty = p.m == -INFINITY && p.l == 0.f;
-        if (a.entropy) a.entropy[row] = empty ? 0.f : log_l - p.s / p.l;
+        if (a.entropy) a.entropy[row] = empty ? 0.f : log_l - p.s / p.l * kLn2;
         if (a.logprob) {
             const int t = a.target[row];
             const bool ok = t >= 0 && t < a.vocab;
@@ -348,12 +400,9 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(LpArgs a, int c
 template <typename T, bool kTop>
 cudaError_t launch_logprobs(const LpArgs& a, int n_rows, int cluster, cudaStream_t st) {
     auto kernel = logprobs_kernel<T, kTop>;
-    const size_t smem = lp_smem<kTop>();
-    if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), (int)smem)) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n_rows * (unsigned)cluster);
     cfg.blockDim = dim3(kLpThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -384,10 +433,10 @@ extern "C" int glm_cuda_logprobs_async(const void* logits_dev, int type, int64_t
     if (top_k > 0 && (!top_ids_dev || !top_logprobs_dev)) return op_fail(GLM_CUDA_ERR_ARG, fn, "top_k=%d without its outputs", top_k);
     int sms = 0;
     if (cudaError_t e = current_sms(&sms)) return launch_failed(fn, e);
-    // CTAs to a row: the most that leave no more CTAs than SMs, up to the
-    // portable cluster size
+    // CTAs to a row: the most that leave no more CTAs than the GPU holds at
+    // once, up to the portable cluster size
     int cluster = 1;
-    while (cluster < kLpMaxCluster && (long long)n_rows * cluster * 2 <= sms) cluster *= 2;
+    while (cluster < kLpMaxCluster && (long long)n_rows * cluster * 2 <= (long long)sms * kLpCtas) cluster *= 2;
     LpArgs a{logits_dev, row_stride, vocab, top_k, target_dev, logprob_dev, entropy_dev, top_ids_dev, top_logprobs_dev};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     try {

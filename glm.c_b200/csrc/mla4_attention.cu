@@ -21,10 +21,10 @@
 // words in shared memory straight into fragments: four bits put into the
 // mantissa of 1024 are 1024 + u (or 1024 + 16 u), and one packed operation
 // makes it v = u - 8, exactly, two values at a time. The query is exact in f16
-// after a power of two per head. The probabilities are rounded to f16 (11
-// bits): p is held relative to a reference within e^4 of its running maximum,
+// after a power of two per head. The probabilities, held relative to a
+// reference within e^4 of their running maximum, are rounded to f16 (11 bits),
 // and once more when a scale is multiplied in: 2^-12 of the position's own
-// weight each time, which is below the output's rounding.
+// weight each time, below the output's rounding.
 //
 // Scales. A position has one scale per 128 latents. The first product ends at
 // each group and is multiplied into the score; for the second a group's sum
