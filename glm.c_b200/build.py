@@ -19,7 +19,7 @@ LIB = os.path.join(PKG, "libglm_cuda.so")
 
 SOURCES = ["glm_cuda.cu", "moe_decode.cu", "moe_persistent.cu", "q80_matvec.cu", "moe_noalloc.cu", "decoder.cu", "moe_prefill.cu", "checkpoint.cu",
            "serve_common.cu", "kv_plan.cu", "kv4_cache.cu", "mla4_attention.cu", "logprobs.cu"]
-HEADERS = ["glm_internal.h", "q80_common.cuh", "route_common.cuh", "glm_cuda.map", "serve_common.h", "kv4.cuh"]
+HEADERS = ["glm_internal.h", "q80_common.cuh", "route_common.cuh", "glm_cuda.map", "serve_common.h", "kv4.cuh", "vec16.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

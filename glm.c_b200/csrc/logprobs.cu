@@ -16,7 +16,7 @@
 // value, which it keeps anyway. The k-th largest of a CTA's threads' largest
 // is no larger than the k-th largest value of its part of the row, so what can
 // be among the best lies in the threads whose largest reaches it, k of them
-// unless there are ties. Their values, one in 256 / k, are read again, and
+// unless there are ties. Their values, one in 512 / k, are read again, and
 // those that reach the bound collect in shared memory and enter a warp's
 // sorted list of 32 (one to a lane, as 64-bit keys: ordered value bits, then
 // the complement of the index, so that ties go to the lowest index) 32 at a
@@ -26,11 +26,15 @@
 // A row is one CTA's, or a thread-block cluster's when there are fewer rows
 // than the GPU holds CTAs; the CTAs of a cluster meet in distributed shared
 // memory. No workspace, no second launch.
+//
+// Measured: 64 rows of 154880 fp32 with the best 20: 15.0 us, of which a launch
+// by itself is about 8 and the reading 6; 1500 rows of 32003 bf16, no best:
+// 22.9 us, 4.2 TB/s, where the exponentials take half of their unit's time and
+// the starts and ends of 1500 CTAs the rest.
 #include <cfloat>
 #include <cmath>
 #include <climits>
 #include <cstdint>
-#include <type_traits>
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -39,15 +43,22 @@
 #include "glm_internal.h"
 #include "q80_common.cuh"
 #include "serve_common.h"
+#include "vec16.cuh"
 
 namespace glmq {
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpWarps = kLpThreads / 32;
+// Threads of a CTA, CTAs that an SM is to hold, 16-byte loads of a thread in
+// flight. The best tokens cost every CTA sorts and merges: fewer, larger CTAs
+// (64 rows of 154880 fp32: 15.0 us, at 256 threads 16.7). Without them more
+// and smaller ones hide the loads (1500 rows of 32003 bf16: 22.9 us, with 4
+// CTAs and 4 loads 24.6, at 512 threads 31).
+template <bool kTop>
+struct LpShape {
+    static constexpr int threads = kTop ? 512 : 256, ctas = kTop ? 2 : 6, vecs = kTop ? 3 : 2, warps = threads / 32;
+};
 constexpr int kLpMaxTop = 32;   // one sorted pair to a lane
 constexpr int kLpMaxCluster = 8;
-constexpr int kLpCtas = 4;      // CTAs an SM holds
 constexpr float kSlack = 8.f;   // a thread's reference may lie this far below its largest value: e^8 in l and s, as floats
 
 struct LpArgs {
@@ -88,27 +99,18 @@ __device__ __forceinline__ Part join(const Part& a, const Part& b) {
     return Part{m, x.l + y.l, x.s + y.s};
 }
 
-// Two fp32 values side by side, for the packed instructions.
-struct Two {
-    unsigned long long v;
-    __device__ __forceinline__ Two() {}
-    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};\n" : "=l"(v) : "f"(a), "f"(b)); }
-    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ Two add2(Two a, Two b) {
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
+// The parts of every kLanes lanes, relative to the largest of their values; top >= p.m is the lane's.
+template <int kLanes>
+__device__ __forceinline__ Part join_lanes(Part p, float top) {
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    p = rebase(p, top);
+#pragma unroll
+    for (int off = kLanes / 2; off > 0; off >>= 1) {
+        p.l += __shfl_xor_sync(0xffffffffu, p.l, off);
+        p.s += __shfl_xor_sync(0xffffffffu, p.s, off);
+    }
+    return p;
 }
 
 // A thread's sums: even and odd values apart.
@@ -181,46 +183,13 @@ __device__ __forceinline__ K merge32(K a, K b, int lane) {
     return v;
 }
 
-template <typename T>
-struct Vec {
-    static constexpr int n = 16 / sizeof(T);
-    int4 raw;
-    __device__ __forceinline__ void load(const T* p) {
-        asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];\n"
-                     : "=r"(raw.x), "=r"(raw.y), "=r"(raw.z), "=r"(raw.w)
-                     : "l"(p));
-    }
-    __device__ __forceinline__ float get(int i) const {
-        const int w[4] = {raw.x, raw.y, raw.z, raw.w};
-        if constexpr (sizeof(T) == 4) return __int_as_float(w[i]);
-        else if constexpr (std::is_same<T, __half>::value)
-            return __half2float(__ushort_as_half((unsigned short)((unsigned)w[i >> 1] >> (16 * (i & 1)))));
-        else
-            return __int_as_float(i & 1 ? w[i >> 1] & 0xffff0000 : w[i >> 1] << 16);
-    }
-    __device__ __forceinline__ float largest() const {  // NaN aside
-        float t = get(0);
-#pragma unroll
-        for (int i = 1; i < n; ++i) t = fmaxf(t, get(i));
-        return t;
-    }
-};
-
-template <typename T>
-__device__ __forceinline__ float value_of(const T* p, long long i) {
-    if constexpr (sizeof(T) == 4) return p[i];
-    else if constexpr (std::is_same<T, __half>::value) return __half2float(p[i]);
-    else return __bfloat162float(p[i]);
-}
-
-constexpr int kLpVecs = 4;                 // 16-byte loads in flight per thread
 constexpr int kLpBuffer = 32 * 8 + 32;     // one warp's candidates: 32 lanes x 8 values to fewer than 32 left from before
 
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(LpArgs a, int cluster) {
+__global__ void __launch_bounds__(LpShape<kTop>::threads, LpShape<kTop>::ctas) logprobs_kernel(LpArgs a, int cluster) {
     namespace cg = cooperative_groups;
     cg::cluster_group cl = cg::this_cluster();
-    constexpr int V = Vec<T>::n, U = kLpVecs;
+    constexpr int V = Vec<T>::n, U = LpShape<kTop>::vecs, kLpThreads = LpShape<kTop>::threads, kLpWarps = LpShape<kTop>::warps;
     __shared__ Part parts[kLpWarps];
     __shared__ Part cta_part;
     __shared__ unsigned tops[kTop ? kLpThreads : 1];     // per warp its threads' largest, sorted; then the CTA's 32 largest
@@ -272,11 +241,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(LpArgs a,
         sums.follow(fmaxf(best, beside));
         sums.add(beside, -INFINITY);
     }
-    Part p = rebase(sums.part(), fmaxf(fmaxf(best, beside), sums.m));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-        p = join(p, Part{__shfl_xor_sync(0xffffffffu, p.m, off), __shfl_xor_sync(0xffffffffu, p.l, off),
-                         __shfl_xor_sync(0xffffffffu, p.s, off)});
+    Part p = sums.part();
+    p = join_lanes<32>(p, fmaxf(best, beside));
     if (lane == 0) parts[warp] = p;
 
     uint64_t list = 0;  // this lane's entry of the warp's sorted best
@@ -348,11 +314,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(LpArgs a,
         }
     }
     if (warp == 0) {
-        p = parts[lane % kLpWarps];  // every eight lanes of the warp form the same sum
-#pragma unroll
-        for (int off = kLpWarps / 2; off > 0; off >>= 1)
-            p = join(p, Part{__shfl_xor_sync(0xffffffffu, p.m, off), __shfl_xor_sync(0xffffffffu, p.l, off),
-                             __shfl_xor_sync(0xffffffffu, p.s, off)});
+        p = parts[lane % kLpWarps];  // every kLpWarps lanes form the same sum
+        p = join_lanes<kLpWarps>(p, p.m);
         if (lane == 0) cta_part = p;
     }
     if (cluster > 1) {
@@ -402,7 +365,7 @@ cudaError_t launch_logprobs(const LpArgs& a, int n_rows, int cluster, cudaStream
     auto kernel = logprobs_kernel<T, kTop>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)n_rows * (unsigned)cluster);
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(LpShape<kTop>::threads);
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -436,7 +399,8 @@ extern "C" int glm_cuda_logprobs_async(const void* logits_dev, int type, int64_t
     // CTAs to a row: the most that leave no more CTAs than the GPU holds at
     // once, up to the portable cluster size
     int cluster = 1;
-    while (cluster < kLpMaxCluster && (long long)n_rows * cluster * 2 <= (long long)sms * kLpCtas) cluster *= 2;
+    const long long held = (long long)sms * (top_k ? LpShape<true>::ctas : LpShape<false>::ctas);
+    while (cluster < kLpMaxCluster && (long long)n_rows * cluster * 2 <= held) cluster *= 2;
     LpArgs a{logits_dev, row_stride, vocab, top_k, target_dev, logprob_dev, entropy_dev, top_ids_dev, top_logprobs_dev};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     try {
