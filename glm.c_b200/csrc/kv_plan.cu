@@ -17,7 +17,11 @@
 // between CTAs and nothing to wait for), then takes its share of the tokens
 // and of the fresh pages, finding a token's request by bisection in shared
 // memory. Tokens are shared out evenly however unevenly the requests hold
-// them.
+// them. Lengths stay below 2^32, so page numbers are 32-bit quotients.
+//
+// Bound by its launch and a chain of four dependent steps (lengths, their sums,
+// a token's request, its page): 256 requests of a token each, or 1021 of up to
+// 300, both 9 us with the launch.
 #include <climits>
 #include <cstdint>
 
@@ -30,11 +34,13 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxReq = 16384;
-constexpr int kPlanTokens = 4;  // consecutive tokens a thread writes together
+constexpr int kPlanTokens = 2;  // consecutive tokens a thread writes together
 
 struct PlanArgs {
     const int32_t *cached, *fresh;
-    int n_req, page, n_free, stride, max_tokens;
+    int n_req;
+    unsigned page;
+    int n_free, stride, max_tokens;
     const int32_t* free_pages;
     int32_t* table;
     int64_t* slots;
@@ -59,7 +65,11 @@ __device__ __forceinline__ Sums warp_scan(Sums v, int lane) {
 
 __device__ __forceinline__ int saturate(long long v) { return v > INT_MAX ? INT_MAX : (int)v; }
 
-__device__ __forceinline__ long long pages_of(long long n, int page) { return (n + page - 1) / page; }
+// ceil(n / page) in 32 bits: lengths and their sums stay below 2^32
+__device__ __forceinline__ unsigned pages_of(unsigned n, unsigned page) {
+    const unsigned q = n / page;
+    return q + (n != q * page);
+}
 
 // Last i in [0, n) with s[i] <= v, for s[0] = 0 <= v: the entry that holds v.
 __device__ __forceinline__ int holder(const int* s, int n, int v) {
@@ -77,7 +87,8 @@ __device__ __forceinline__ int holder(const int* s, int n, int v) {
 __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     extern __shared__ int plan_sm[];
     int* start = plan_sm;                 // [n_req + 1] first token of each request
-    int* first = plan_sm + a.n_req + 1;   // [n_req + 1] first fresh page of each request
+    int* first = start + a.n_req + 1;     // [n_req + 1] first fresh page of each request
+    int* held = first + a.n_req + 1;      // [n_req] positions in pages already held
     __shared__ Sums warp_tot[kPlanThreads / 32];
     __shared__ int status_bits;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -92,10 +103,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     for (int r = r0; r < r1; ++r) {
         const int c = a.cached[r], n = a.fresh[r];
         if (c < 0 || n < 0) bits |= 8;
-        const long long cc = max(c, 0), nn = max(n, 0);
-        if (pages_of(cc + nn, a.page) > a.stride) bits |= 2;
+        const unsigned cc = max(c, 0), nn = max(n, 0), pages = pages_of(cc + nn, a.page);
+        if (pages > (unsigned)a.stride) bits |= 2;
+        held[r] = (int)cc;
         mine.tokens += nn;
-        mine.pages += pages_of(cc + nn, a.page) - pages_of(cc, a.page);
+        mine.pages += pages - pages_of(cc, a.page);
     }
     Sums run = warp_scan(mine, lane);
     if (lane == 31) warp_tot[warp] = run;
@@ -114,7 +126,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     for (int r = r0; r < r1; ++r) {
         start[r] = saturate(at.tokens);
         first[r] = saturate(at.pages);
-        const long long cc = max(a.cached[r], 0), nn = max(a.fresh[r], 0);
+        if (r + 1 == r1) break;  // the next thread's, or the total
+        const unsigned cc = held[r], nn = max(a.fresh[r], 0);
         at.tokens += nn;
         at.pages += pages_of(cc + nn, a.page) - pages_of(cc, a.page);
     }
@@ -138,7 +151,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
     // fresh pages into their requests' tables; past the free list: -1
     for (long long k = gtid; k < n_fresh; k += gthreads) {
         const int i = holder(first, a.n_req, (int)k);
-        const long long col = pages_of(max(a.cached[i], 0), a.page) + (k - first[i]);
+        const long long col = pages_of(held[i], a.page) + (k - first[i]);
         if (col < a.stride) a.table[(size_t)i * a.stride + col] = k < a.n_free ? a.free_pages[k] : -1;
     }
 
@@ -154,18 +167,20 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(PlanArgs a) {
             pos[u] = req[u] = -1;
             if (j < n_tokens && j < a.max_tokens) {
                 while (start[i + 1] <= j) ++i;  // requests without tokens are stepped over
-                const long long c = max(a.cached[i], 0), p = c + (j - start[i]);
-                const long long col = p / a.page, held = pages_of(c, a.page);
+                const unsigned c = held[i], p = c + (unsigned)(j - start[i]);
+                const unsigned col = p / a.page, old = pages_of(c, a.page);
                 int id = -1;
-                if (col < held) {
-                    if (col < a.stride) id = a.table[(size_t)i * a.stride + col];
-                } else if (col < a.stride) {
-                    const long long k = first[i] + (col - held);
-                    if (k < a.n_free) id = a.free_pages[k];
+                if (col < (unsigned)a.stride) {
+                    if (col < old) {
+                        id = a.table[(size_t)i * a.stride + col];
+                    } else {
+                        const unsigned k = (unsigned)first[i] + (col - old);
+                        if (k < (unsigned)a.n_free) id = a.free_pages[k];
+                    }
                 }
-                pos[u] = saturate(p);
+                pos[u] = saturate((long long)p);
                 req[u] = i;
-                if (id >= 0) slot[u] = (int64_t)id * a.page + (p - col * a.page);
+                if (id >= 0) slot[u] = (int64_t)id * a.page + (int64_t)(p - col * a.page);
             }
         }
 #pragma unroll
@@ -197,13 +212,13 @@ extern "C" int glm_cuda_kv_plan_async(const int32_t* cached_len_dev, const int32
         return op_fail(GLM_CUDA_ERR_ARG, fn, "max_tokens=%d without its outputs", max_tokens);
     int sms = 0;
     if (cudaError_t e = current_sms(&sms)) return launch_failed(fn, e);
-    const size_t smem = 2 * sizeof(int) * ((size_t)n_req + 1);
+    const size_t smem = sizeof(int) * (3 * (size_t)n_req + 2);
     const long long items = (long long)kPlanThreads * kPlanTokens;
     long long grid = (max_tokens + items - 1) / items;
     grid = grid < 1 ? 1 : grid > sms ? sms : grid;
     try {
         cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kv_plan_kernel), (int)smem);
-        PlanArgs a{cached_len_dev, new_len_dev, n_req, page_size, n_free, table_stride, max_tokens, free_pages_dev,
+        PlanArgs a{cached_len_dev, new_len_dev, n_req, (unsigned)page_size, n_free, table_stride, max_tokens, free_pages_dev,
                    block_table_dev, slot_map_dev, positions_dev, token_req_dev, token_start_dev, summary_dev};
         if (!e) e = launch_pdl(kv_plan_kernel, (unsigned)grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
         if (e) return launch_failed(fn, e);
