@@ -21,7 +21,7 @@
 //
 // Bound by its launch and a chain of four dependent steps (lengths, their sums,
 // a token's request, its page): 256 requests of a token each, or 1021 of up to
-// 300, both 9 us with the launch.
+// 391, both 9 us with the launch.
 #include <climits>
 #include <cstdint>
 

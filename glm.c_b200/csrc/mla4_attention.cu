@@ -42,17 +42,21 @@
 // (cp.async.bulk, completion on mbarriers). Warps 0-7 take a unit of 32
 // positions each in turn: scores, references, the probabilities in f16. Warps
 // 8-15 own 64 latents each: the second product of every tile. The two kinds
-// split the registers (112 a thread) and run on different tiles, so one's
-// products cover the other's unpacking and exponentials.
+// split the registers (120 and 104 a thread) and run on different tiles, so
+// one's products cover the other's unpacking and exponentials. A tile's stage
+// and its probabilities' buffers are free again when its sums are done: one
+// barrier for both.
 //
 // What bounds it, measured at 16 requests of 32768 positions, 20 heads of 512 +
-// 64 (153 MB of cache): 132 us, 1.16 TB/s. The products take 43 % of the tensor
+// 64 (153 MB of cache): 128 us, 1.19 TB/s. The products take 43 % of the tensor
 // pipe's time, the instructions around them (unpacking, scales, waits) keep 53 %
-// of the issue slots; 16 warps of 112 registers are all that an SM holds, too
+// of the issue slots; 16 such warps are all that an SM holds, too
 // few to fill the rest. At one request of 1500 positions it takes 21 us, most
 // of it three dependent steps: the query's load, one tile a CTA, the join.
 // Tried on the way here and slower at that size: 12 score and 4 sum warps (200
 // us: spills), the sum warps in units of 32 positions (137 us: a wait for each),
+// the codes as f16 numbers below 2^-14, unbiased by -8 times the query's sum
+// (137 us, and four times the error in scores of hundreds),
 // tcgen05 with the codes spread to bytes in shared memory (192 us: the warps
 // that spread the codes and read the accumulators back are the bound).
 // m16n8k32 e4m3, for which the codes need no arithmetic, issues at 0.21 a clock
@@ -77,6 +81,7 @@ namespace {
 constexpr int kTile = 64;                 // positions that are copied together
 constexpr int kUnit = 32;                 // positions that a score warp takes together
 constexpr int kScoreWarps = 8, kSumWarps = 8;
+constexpr int kPairs = kScoreWarps / (kTile / kUnit);  // tiles whose probabilities are kept
 constexpr float kRaise = 4.f, kRaiseScale = 16.f;
 constexpr int kProducer = kScoreWarps + kSumWarps;
 constexpr int kAtThreads = 640;           // warpgroups: two of scores, two of sums, one of which a warp copies
@@ -200,8 +205,9 @@ __device__ __forceinline__ float exp_of(float d) {
 
 // Registers of the calling warpgroup's threads. The launch has 96 for each of
 // 640 threads, 5 x 96 = 480 over a thread of every group; the groups' shares
-// are 32 + 2 x 112 + 2 x 112.
-constexpr int kCopyRegs = 32, kScoreRegs = 112, kSumRegs = 112;
+// are 32 + 2 x 120 + 2 x 104: the scores spill without the eight more (112 each: 2 %
+// slower at the longest case, 104 for the scores 20 %).
+constexpr int kCopyRegs = 32, kScoreRegs = 120, kSumRegs = 104;
 static_assert(kCopyRegs + 2 * kScoreRegs + 2 * kSumRegs <= 5 * 96, "more registers than the launch has");
 template <int kRegs>
 __device__ __forceinline__ void shrink_registers() {
@@ -214,7 +220,8 @@ __device__ __forceinline__ void grow_registers() {
 
 // A bounded wait whose outcome is the whole warp's.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity));
+    // (woken by the barrier, where a first look that fails would read the clock)
+    return __all_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, kSuspendNs) || mbar_wait_bounded(bar, parity));
 }
 
 // Positions that row `row` sees.
@@ -354,9 +361,9 @@ __device__ __forceinline__ int swizzled(int u, int row) { return u ^ (4 * (row >
 template <int NT>
 __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm, const Smem<NT>& L, int warp, int lane,
                                            const unsigned char* rows, const unsigned char* scales, int scale_step,
-                                           const unsigned char* query, uint32_t seen, bool first, uint64_t* empty,
+                                           const unsigned char* query, uint32_t seen, bool first,
                                            uint64_t* chain_before, uint32_t chain_parity, uint64_t* chain_mine,
-                                           uint64_t* prob_empty, uint32_t prob_parity) {
+                                           uint64_t* summed, uint32_t summed_parity) {
     const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes(), groups = a.sh.groups();
     float* ss = reinterpret_cast<float*>(sm + L.scratch + warp * L.kScaleBytes);  // [group][4 g + j]
     float* stats = reinterpret_cast<float*>(sm + L.stats) + warp * L.kStats;
@@ -443,8 +450,6 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
     products(2 * (groups - 1), true);
     if (a.sh.rope > 64) products(2 * groups - 1, false);
     scaled(groups - 1);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(empty);  // codes and scales of this unit are read
 
     // scores, and the lane's largest of each head
     const float* factor = reinterpret_cast<const float*>(query + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
@@ -463,8 +468,15 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
             }
     }
 
+    float tallest[4];  // of the unit's scales
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr)
+        if (gr < groups - 1)
+            tallest[gr] = __uint_as_float(__reduce_max_sync(0xffffffffu, scale[gr] == 0x7fc00000u ? 0u : scale[gr]));
+
     // the references, from the unit before (the item's first waits too: the
-    // last item's must have been read)
+    // last item's must have been read). Every unit's turn at them is one after
+    // the other's: most have nothing to change and pass them on at once.
     if (chain_before && !warp_wait(chain_before, chain_parity)) return false;
     bool moved = false;
 #pragma unroll
@@ -475,8 +487,14 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
         // (a head that has seen nothing yet takes whatever comes)
         moved |= top[n][0] > was.x + kRaise || top[n][1] > was.y + kRaise;
     }
-    moved = __any_sync(0xffffffffu, moved);
-    if (moved) {  // some head's largest of the unit is above its reference by more than that
+    float ref[4];
+#pragma unroll
+    for (int gr = 0; gr < 4; ++gr) {
+        ref[gr] = first ? 0.f : chain[8 * NT + gr];
+        if (gr < groups - 1) moved |= tallest[gr] > kRaiseScale * ref[gr];
+    }
+    moved = __any_sync(0xffffffffu, moved || first);
+    if (moved) {  // some head's largest of the unit is above its reference by more than that, or a scale
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -485,27 +503,18 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
                 for (int off = 4; off < 32; off <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(0xffffffffu, top[n][e], off));
                 if (top[n][e] > R[n][e] + kRaise) R[n][e] = top[n][e];
             }
-    }
-    float ref[4];
 #pragma unroll
-    for (int gr = 0; gr < 4; ++gr) {
-        ref[gr] = first ? 0.f : chain[8 * NT + gr];
-        if (gr < groups - 1) {
-            const uint32_t top = __reduce_max_sync(0xffffffffu, scale[gr] == 0x7fc00000u ? 0u : scale[gr]);
-            if (__uint_as_float(top) > kRaiseScale * ref[gr]) {
-                ref[gr] = __uint_as_float(((top >> 23) + 1) << 23);
-                moved = true;
-            }
+        for (int gr = 0; gr < 4; ++gr)
+            if (gr < groups - 1 && tallest[gr] > kRaiseScale * ref[gr])
+                ref[gr] = __uint_as_float(((__float_as_uint(tallest[gr]) >> 23) + 1) << 23);
+        __syncwarp();
+        if (g == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(chain + 8 * n + 2 * t) = make_float2(R[n][0], R[n][1]);
+            if (t == 0) *reinterpret_cast<float4*>(chain + 8 * NT) = make_float4(ref[0], ref[1], ref[2], ref[3]);
         }
+        __syncwarp();
     }
-    moved |= first;
-    __syncwarp();
-    if (moved && g == 0) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(chain + 8 * n + 2 * t) = make_float2(R[n][0], R[n][1]);
-        if (t == 0) *reinterpret_cast<float4*>(chain + 8 * NT) = make_float4(ref[0], ref[1], ref[2], ref[3]);
-    }
-    __syncwarp();
     if (lane == 0) mbar_arrive(chain_mine);
 
     __half2 ph[NT][2][2];
@@ -529,7 +538,7 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
-    if (!warp_wait(prob_empty, prob_parity)) return false;
+    if (summed && !warp_wait(summed, summed_parity)) return false;
     if (g == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -573,31 +582,32 @@ __device__ __forceinline__ int column_head(int n, int r) { return 8 * n + 2 * (r
 
 // What a sum warp carries through an item: lane (g, t) holds latents
 // 8 g + (2 b, 2 b + 1) of its 64, of the columns 2 t and 2 t + 1, in
-// units of ref and relative to R.
+// units of ref and relative to R; R and L are those of column `lane`.
 template <int NT>
 struct Sum {
-    float O[4][NT][4], R[NT][2], L[NT][2], ref;
+    float O[4][NT][4], R, L, ref;
 };
 
 // The references a unit was scored with, where they have moved.
 template <int NT>
-__device__ __forceinline__ void follow(Sum<NT>& s, int group, int t, const float* stats) {
+__device__ __forceinline__ void follow(Sum<NT>& s, int group, int lane, const float* stats) {
     if (stats[16 * NT + 4] == 0.f) return;
     const float ref = stats[16 * NT + group];
     const float step = ref > 0.f ? s.ref / ref : 0.f;
     s.ref = ref;
+    const float R = lane < 8 * NT ? stats[lane] : 0.f;
+    const float al = s.R == -INFINITY ? 0.f : exp_of(s.R - R);
+    s.R = R;
+    s.L *= al;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float R = stats[8 * n + 2 * t + e];
-            const float al = s.R[n][e] == -INFINITY ? 0.f : exp_of(s.R[n][e] - R);
-            s.R[n][e] = R;
-            s.L[n][e] *= al;
+            const float by = __shfl_sync(0xffffffffu, al, 8 * n + 2 * (lane & 3) + e) * step;
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
-                s.O[b][n][e] *= al * step;
-                s.O[b][n][2 + e] *= al * step;
+                s.O[b][n][e] *= by;
+                s.O[b][n][2 + e] *= by;
             }
         }
 }
@@ -631,13 +641,8 @@ __device__ __forceinline__ void sum_tile(const Mla4Args& a, Sum<NT>& s, int grou
     for (int st = 0; st < kSteps; ++st) {
         if (st % (kSteps / kUnits) == 0) {
             const float* u = stats + st / (kSteps / kUnits) * Smem<NT>::kStats;
-            follow<NT>(s, group, t, u);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float2 l = *reinterpret_cast<const float2*>(u + 8 * NT + 8 * n + 2 * t);
-                s.L[n][0] += l.x;
-                s.L[n][1] += l.y;
-            }
+            follow<NT>(s, group, lane, u);
+            if (lane < 8 * NT) s.L += u[8 * NT + lane];
         }
         const Step& f = at[st & 1];
         if (st + 1 < kSteps) fetch(st + 1, at[(st + 1) & 1]);
@@ -701,8 +706,8 @@ __device__ __forceinline__ void finish_item(const Mla4Args& a, const Sum<NT>& s,
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int c = column_head(n, 2 * t + e);
+            const float L = __shfl_sync(0xffffffffu, s.L, 8 * n + 2 * t + e), R = __shfl_sync(0xffffffffu, s.R, 8 * n + 2 * t + e);
             if (c >= a.block_heads || h0 + c >= a.n_heads) continue;
-            const float L = s.L[n][e], R = s.R[n][e];
             const float unit = s.ref * (whole && L != 0.f ? 1.f / L : 1.f);
             float v[8];
 #pragma unroll
@@ -731,7 +736,7 @@ __device__ __forceinline__ void finish_item(const Mla4Args& a, const Sum<NT>& s,
 template <int NT, bool kBf16>
 __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args a) {
     extern __shared__ __align__(128) unsigned char sm[];
-    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], prob_full[kScoreWarps], prob_empty[kScoreWarps],
+    __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], prob_full[kPairs],
         chain[kScoreWarps], query_full[2], query_empty[2];
     __shared__ uint64_t seen[kMaxStages];  // positions of the stage's tile that the row sees
     __shared__ long long scan[kAtThreads / 32 + 1];
@@ -742,13 +747,10 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
     if (tid == 0) {
         for (int i = 0; i < a.stages; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], kTile / kUnit + kSumWarps);
+            mbar_init(&empty[i], kSumWarps);
         }
-        for (int i = 0; i < kScoreWarps; ++i) {
-            mbar_init(&prob_full[i], 1);
-            mbar_init(&prob_empty[i], kSumWarps);
-            mbar_init(&chain[i], 1);
-        }
+        for (int i = 0; i < kPairs; ++i) mbar_init(&prob_full[i], kTile / kUnit);
+        for (int i = 0; i < kScoreWarps; ++i) mbar_init(&chain[i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&query_full[i], kScoreWarps);
             mbar_init(&query_empty[i], kScoreWarps);
@@ -923,11 +925,13 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
                     // this lane's position: its scales lie `per` apart from group to group
                     const unsigned pos = p0 + lane;
                     const unsigned char* scales = tile + kTile * rb + 2 * ((pos >> per_log) * groups * per + (pos & (per - 1)));
+                    // its probabilities take the place of the tile's kPairs before
+                    const int old = at.stage < kPairs ? at.stage + stages - kPairs : at.stage - kPairs;
                     ok = score_unit<NT>(a, sm, L, warp, lane, tile + p0 * rb, scales, 2 * per, query,
-                                        (uint32_t)(seen[at.stage] >> p0), mine == u0, &empty[at.stage],
+                                        (uint32_t)(seen[at.stage] >> p0), mine == u0,
                                         mine ? &chain[(mine - 1) % kScoreWarps] : nullptr, (mine - 1) / kScoreWarps & 1,
-                                        &chain[warp], &prob_empty[warp], (mine / kScoreWarps & 1) ^ 1);
-                    if (ok && lane == 0) mbar_arrive(&prob_full[warp]);
+                                        &chain[warp], mine >= kScoreWarps ? &empty[old] : nullptr, at.phase ^ (at.stage < kPairs));
+                    if (ok && lane == 0) mbar_arrive(&prob_full[warp / kUnits]);
                     if (!ok) break;
                 }
                 if (!loaded && more) {
@@ -953,33 +957,25 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
         Place at;
         while (ok && w.next()) {
             Sum<NT> s;
-            s.ref = 0.f;
+            s.ref = s.L = 0.f;
+            s.R = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int b = 0; b < 4; ++b)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    s.R[n][e] = -INFINITY;
-                    s.L[n][e] = 0.f;
-                }
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s.O[b][n][r] = 0.f;
-            }
-            for (int tile = w.first; tile < w.end; ++tile, at.forward(1, stages), u += kTile / kUnit) {
-                static_assert(kTile == 2 * kUnit && kScoreWarps % 2 == 0, "a tile's two units lie in neighbouring buffers");
-                const unsigned buf = u % kScoreWarps, parity = u / kScoreWarps & 1;
-                const bool here = mbar_wait_bounded(&full[at.stage], at.phase) && mbar_wait_bounded(&prob_full[buf], parity) &&
-                                  mbar_wait_bounded(&prob_full[buf + 1], parity);
-                ok = __all_sync(0xffffffffu, here);
+            for (int tile = w.first; tile < w.end; ++tile, at.forward(1, stages), ++u) {
+                // the tile's codes are there too: its scores were formed from them
+                const unsigned pair = u % kPairs;
+                ok = warp_wait(&prob_full[pair], u / kPairs & 1);
                 if (!ok) break;
-                const unsigned char* probs = sm + L.probs + buf * L.kProbBytes;
+                const unsigned char* probs = sm + L.probs + pair * (kTile / kUnit) * L.kProbBytes;
                 if (works)
                     sum_tile<NT>(a, s, group, lane, sm + L.ring + at.stage * L.stage + part * 32, probs, probs + L.kRatios + group * kUnit * 2,
-                                 reinterpret_cast<const float*>(sm + L.stats) + buf * L.kStats);
+                                 reinterpret_cast<const float*>(sm + L.stats) + pair * (kTile / kUnit) * L.kStats);
                 __syncwarp();
-                if (lane < 2) mbar_arrive(&prob_empty[buf + lane]);
-                if (lane == 2) mbar_arrive(&empty[at.stage]);
+                if (lane == 0) mbar_arrive(&empty[at.stage]);
             }
             if (ok && works) finish_item<NT, kBf16>(a, s, w, part, lane);
         }
@@ -1086,7 +1082,7 @@ template <int NT, bool kBf16>
 cudaError_t launch_attention(Mla4Args a, int ctas, cudaStream_t st) {
     constexpr int kMost = 225 * 1024;
     a.stages = kMaxStages;
-    while (a.stages > 2 && Smem<NT>(a.sh, a.stages).bytes > kMost) --a.stages;
+    while (a.stages > kPairs && Smem<NT>(a.sh, a.stages).bytes > kMost) --a.stages;
     const int smem = Smem<NT>(a.sh, a.stages).bytes;
     auto kernel = mla4_attention_kernel<NT, kBf16>;
     if (cudaError_t e = ensure_smem_attr(reinterpret_cast<const void*>(kernel), smem)) return e;
