@@ -1,0 +1,138 @@
+"""Many requests over one pool of 4-bit latent pages: the operators of include/glm_cuda.h's serving section, in the
+order in which a decoder uses them.
+
+    pool = LatentPool(lib, layers, n_pages, kv_lora, rope, page_size, max_req, max_len)
+    pool.open(r)                                  # request r, without positions yet
+    step = pool.plan({r: 7, s: 1})                # 7 new tokens of r, one of s
+    for layer in range(layers):
+        pool.store(layer, step, latent, k_pe)     # the new tokens' cache rows
+        ctx = pool.attend(layer, step, q, scale)  # each over its request's positions up to its own
+    pool.scores(logits, target, k)                # log probabilities, entropies, most likely tokens
+
+glm.c serves one sequence from one contiguous fp32 cache (infer.c:1003-1058, 1218-1290, 2190-2228); a request here
+holds pages of the pool instead, given out in request order and taken back by close().
+"""
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+
+def _stream() -> int:
+    """Everything runs on torch's current stream, on which its tensors may also be freed."""
+    return torch.cuda.current_stream().cuda_stream
+
+
+@dataclasses.dataclass
+class Step:
+    """A step's new tokens, request after request: device tensors of `tokens` entries each."""
+
+    requests: list[int]   # in the order of their tokens
+    tokens: int
+    slots: torch.Tensor   # int64
+    req: torch.Tensor     # int32, the token's row of the pool's block table
+    pos: torch.Tensor     # int32
+    last: torch.Tensor    # int64, the index of every request's last token
+
+
+class LatentPool:
+    """Pages of every layer's cache (a page id is the same page in all of them), block tables and lengths."""
+
+    def __init__(self, lib, layers: int, n_pages: int, kv_lora: int, rope: int, page_size: int, max_req: int, max_len: int):
+        self.lib, self.page_size, self.kv_lora, self.rope = lib, page_size, kv_lora, rope
+        size = lib.kv4_page_bytes(kv_lora, rope, page_size)
+        if size == 0:
+            raise ValueError(f"no 4-bit cache of kv_lora {kv_lora}, rope {rope}, page_size {page_size}")
+        self.caches = [lib.kv4_cache(torch.empty(n_pages * size, dtype=torch.uint8, device="cuda"), n_pages, kv_lora, rope,
+                                     page_size) for _ in range(layers)]
+        self.table = torch.full((max_req, -(-max_len // page_size)), -1, dtype=torch.int32, device="cuda")
+        self.free = list(range(n_pages))
+        self.pages: dict[int, list[int]] = {}  # of an open request
+        self.length: dict[int, int] = {}
+        self.max_req, self.max_len = max_req, max_len
+        self._ws = torch.empty(0, dtype=torch.uint8, device="cuda")
+
+    def open(self, request: int) -> None:
+        if not 0 <= request < self.max_req or request in self.length:
+            raise ValueError(f"request {request} is open or not in [0, {self.max_req})")
+        self.pages[request], self.length[request] = [], 0
+
+    def close(self, request: int) -> None:
+        """Its pages go back to the pool. Steps enqueued before still read them; a later step writes after them."""
+        self.free += self.pages.pop(request)
+        del self.length[request]
+
+    def plan(self, new: dict[int, int]) -> Step:
+        """Pages, slots and positions of new[r] tokens of each request r."""
+        counts = [new.get(r, 0) if r in self.length else 0 for r in range(self.max_req)]
+        total, P = sum(counts), self.page_size
+        if total == 0 or sum(new.values()) != total or min(new.values()) < 0:
+            raise ValueError("a step has tokens of open requests")
+        need = {r: -(-(self.length[r] + c) // P) - len(self.pages[r]) for r, c in enumerate(counts) if c}
+        for r, c in enumerate(counts):
+            if c and self.length[r] + c > self.max_len:
+                raise ValueError(f"request {r} would pass {self.max_len} positions")
+        if sum(need.values()) > len(self.free):
+            raise MemoryError(f"{sum(need.values())} pages are needed, {len(self.free)} are free")
+
+        def ints(v):
+            return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+        def empty(n, dtype=torch.int32):
+            return torch.empty(n, dtype=dtype, device="cuda")
+
+        slots, pos, req, start, summary = empty(total, torch.int64), empty(total), empty(total), empty(self.max_req + 1), empty(4)
+        taken = sum(need.values())
+        self.lib.kv_plan_async(ints([self.length.get(r, 0) for r in range(self.max_req)]), ints(counts), P,
+                               ints(self.free[:taken]), self.table, total, slots, pos, req, start, summary, _stream())
+        for r, n in need.items():  # the device gives them out in the same order
+            self.pages[r] += self.free[:n]
+            del self.free[:n]
+            self.length[r] += counts[r]
+        order = [r for r, c in enumerate(counts) if c]
+        return Step(order, total, slots, req, pos, (start[1:][torch.tensor(order, device="cuda")] - 1).long())
+
+    def store(self, layer: int, step: Step, latent, k_pe) -> None:
+        self.lib.kv4_store_async(self.caches[layer], latent, k_pe, step.slots, _stream())
+
+    def attend(self, layer: int, step: Step, q, scale: float):
+        """Context latents [tokens, heads, kv_lora] of the absorbed queries q [tokens, heads, kv_lora + rope]."""
+        out = torch.empty(*q.shape[:2], self.kv_lora, dtype=q.dtype, device="cuda")
+        need = self.lib.mla4_workspace_bytes(q.shape[0], q.shape[1], self.kv_lora)
+        if self._ws.numel() < need:
+            self._ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        self.lib.mla4_attention_async(self.caches[layer], q, self.table, step.req, step.pos, scale, out, None, self._ws, _stream())
+        return out
+
+    def scores(self, logits, target=None, k: int = 0):
+        """(log probability of target or None, entropy, top ids or None, their log probabilities or None) per row."""
+        n = logits.shape[0]
+        f32 = dict(dtype=torch.float32, device="cuda")
+        logprob = torch.empty(n, **f32) if target is not None else None
+        entropy = torch.empty(n, **f32)
+        ids = torch.empty(n, k, dtype=torch.int32, device="cuda") if k else None
+        tops = torch.empty(n, k, **f32) if k else None
+        self.lib.logprobs_async(logits, target, logprob, entropy, ids, tops, _stream())
+        return logprob, entropy, ids, tops
+
+    def rows(self, layer: int, request: int, first: int = 0, end: int | None = None, dtype=torch.float32):
+        """Cached rows [first, end) of a request as numbers: latents and rope parts."""
+        end = self.length[request] if end is None else end
+        p = torch.arange(first, end)
+        slots = torch.tensor(self.pages[request], dtype=torch.int64)[p // self.page_size] * self.page_size + p % self.page_size
+        latent = torch.empty(end - first, self.kv_lora, dtype=dtype, device="cuda")
+        k_pe = torch.empty(end - first, self.rope, dtype=dtype, device="cuda")
+        self.lib.kv4_load_async(self.caches[layer], slots.cuda(), latent, k_pe, _stream())
+        return latent, k_pe
+
+    def fork(self, request: int, to: int) -> None:
+        """Request `to` starts as a copy of `request`. A row read back and stored again keeps its codes and scales:
+        its largest magnitude is 7 times the scale."""
+        n = self.length[request]
+        self.open(to)
+        if n == 0:
+            return
+        step = self.plan({to: n})
+        for layer in range(len(self.caches)):
+            self.store(layer, step, *self.rows(layer, request, 0, n))

@@ -1,0 +1,119 @@
+"""Many requests from prompt to tokens over the paged 4-bit cache: glm.c_b200/serve.py and examples/serve_requests.py.
+
+The attention of a whole run is compared with a plain one in 64 bits over the rows that the cache gives back, and the
+run's bookkeeping with itself: forks, pages taken and returned, requests served alone and together.
+"""
+import importlib
+import os
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib(pkg):
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    pkg.build.build()
+    return pkg.glm_cuda.GlmCuda()
+
+
+@pytest.fixture(scope="module")
+def pool_type(pkg):
+    return importlib.import_module(pkg.__name__ + ".serve").LatentPool
+
+
+@pytest.fixture(scope="module")
+def example():
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import serve_requests
+
+    return serve_requests
+
+
+def prompts_of(*lengths):
+    g = torch.Generator().manual_seed(3)
+    return [torch.randint(5003, (n,), generator=g).tolist() for n in lengths]
+
+
+def test_every_attention_of_a_run_against_64_bits(lib, pool_type, example):
+    # bf16 output 2^-9 relative at most and probabilities of no fewer than 8 bits, as for the operator itself: 4e-3 of
+    # the row's norm
+    seen = []
+
+    class Checked(pool_type):
+        def attend(self, layer, step, q, scale):
+            out = super().attend(layer, step, q, scale)
+            for i in range(step.tokens):
+                r, n = int(step.req[i]), int(step.pos[i]) + 1
+                latent, k_pe = (t.double() for t in self.rows(layer, r, 0, n))
+                p = torch.softmax(scale * (q[i].double() @ torch.cat([latent, k_pe], 1).T), 1)
+                ref = p @ latent
+                seen.append(float(((out[i].double() - ref).norm(dim=1) / ref.norm(dim=1)).max()))
+            return out
+
+    result, pool, model = example.serve(lib, Checked, prompts_of(1, 21, 40), 4, fork_at=2)
+    assert len(seen) == model.layers * (1 + 21 + 40 + 3 + 3 + 4)  # the prompts, two steps of three requests, one of four
+    assert max(seen) <= 4e-3
+    for out in result.values():
+        assert len(out["tokens"]) == out["prompt"] + 4
+        for lp, (_, other) in zip(out["logprobs"], out["alternatives"]):
+            assert lp < 0 and other < 0
+        assert all(lp < 0 for lp in out["prompt_logprobs"]) and len(out["prompt_logprobs"]) == out["prompt"] - 1
+
+
+def test_a_fork_is_a_copy(lib, pool_type):
+    pool = pool_type(lib, 2, 40, 128, 64, 16, 3, 200)
+    pool.open(0)
+    pool.open(1)
+    g = torch.Generator("cuda").manual_seed(5)
+    for n in (100, 1, 30):
+        step = pool.plan({0: n, 1: 3})
+        for layer in range(2):
+            pool.store(layer, step, torch.randn(n + 3, 128, generator=g, device="cuda"),
+                       torch.randn(n + 3, 64, generator=g, device="cuda"))
+    pool.fork(0, 2)
+    assert pool.length == {0: 131, 1: 9, 2: 131} and not set(pool.pages[0]) & set(pool.pages[2])
+    size = lib.kv4_page_bytes(128, 64, 16)
+    for layer in range(2):
+        for a, b in zip(pool.rows(layer, 0), pool.rows(layer, 2)):
+            assert torch.equal(a, b) and a.abs().max() > 0
+        raw = pool.caches[layer].tensor.view(-1, size)
+        whole = 131 // 16
+        assert torch.equal(raw[pool.pages[0][:whole]], raw[pool.pages[2][:whole]])
+
+
+def test_together_as_alone(lib, pool_type, example):
+    # a row's attention depends on its own positions alone; torch's products may differ in the last bit with the number
+    # of rows, so log probabilities agree to bf16 logits of size 8 or so: 2^-8 * 8, doubled
+    prompts = prompts_of(33, 5, 64)
+    together, _, _ = example.serve(lib, pool_type, prompts, 1)
+    for r, p in enumerate(prompts):
+        alone, _, _ = example.serve(lib, pool_type, [p], 1)
+        a, b = torch.tensor(alone[0]["prompt_logprobs"]), torch.tensor(together[r]["prompt_logprobs"])
+        assert (a - b).abs().mean() <= 2 ** -4
+
+
+def test_pages_return_and_run_out(lib, pool_type):
+    pool = pool_type(lib, 1, 6, 128, 64, 16, 4, 96)
+    pool.open(0)
+    pool.open(2)
+    pool.plan({0: 40, 2: 17})  # 3 + 2 pages
+    assert len(pool.free) == 1
+    with pytest.raises(MemoryError):
+        pool.plan({2: 33})
+    assert pool.length == {0: 40, 2: 17} and len(pool.free) == 1
+    with pytest.raises(ValueError):
+        pool.plan({1: 1})
+    with pytest.raises(ValueError):
+        pool.open(2)
+    pool.close(0)
+    assert len(pool.free) == 4
+    step = pool.plan({2: 33})
+    assert step.requests == [2] and step.pos.tolist() == list(range(17, 50))
+    held = pool.pages[2]
+    assert step.slots.tolist() == [held[p // 16] * 16 + p % 16 for p in range(17, 50)]
+    with pytest.raises(ValueError):
+        pool.plan({2: 50})
