@@ -218,10 +218,17 @@ __device__ __forceinline__ void grow_registers() {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegs));
 }
 
-// A bounded wait whose outcome is the whole warp's.
+// A bounded wait whose outcome is the whole warp's: woken by the barrier, or
+// given up after kWaitNs.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-    // (woken by the barrier, where a first look that fails would read the clock)
-    return __all_sync(0xffffffffu, mbar_try_wait_sleep(bar, parity, kSuspendNs) || mbar_wait_bounded(bar, parity));
+    bool here = mbar_try_wait_sleep(bar, parity, kSuspendNs);
+    if (!here) {
+        const uint64_t t0 = global_ns();
+#pragma unroll 1
+        do here = mbar_try_wait_sleep(bar, parity, kSuspendNs);
+        while (!here && global_ns() - t0 < kWaitNs);
+    }
+    return __all_sync(0xffffffffu, here);
 }
 
 // Positions that row `row` sees.
@@ -240,6 +247,7 @@ struct Place {
     int stage = 0;
     uint32_t phase = 0;
     __device__ __forceinline__ void forward(int tiles, int stages) {
+#pragma unroll 1
         for (stage += tiles; stage >= stages; stage -= stages) phase ^= 1u;
     }
 };
@@ -279,34 +287,33 @@ __device__ __forceinline__ void load_query(const Mla4Args& a, int row, int block
     const int chunks = (a.sh.kv_lora + a.sh.rope) / 8;  // at most 80
     const int h0 = block * a.block_heads;
     float* factor = reinterpret_cast<float*>(qf + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
-    // warp w has the heads w, w + 8, ...: all their loads go out before the first is used
-    if (warp >= 8) return;
-    uint32_t raw[NT][3][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    // warp w has the heads w, w + 8, ...: the next one's values are on their way while one is converted
+    uint32_t raw[3][4];
+    auto fetch = [&](int n) {
         const int c = 8 * n + warp;
-        const bool live = c < a.block_heads && h0 + c < a.n_heads;
+        const bool live = n < NT && c < a.block_heads && h0 + c < a.n_heads;
         const uint16_t* q = static_cast<const uint16_t*>(a.q) + (long long)row * a.q_row + (long long)(h0 + c) * a.q_head;
 #pragma unroll
         for (int u = 0; u < 3; ++u) {
             const int ch = u * 32 + lane;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[n][u][i] = 0u;
+            for (int i = 0; i < 4; ++i) raw[u][i] = 0u;
             if (live && ch < chunks) {
                 if (a.vec) {
                     const uint4 r = __ldg(reinterpret_cast<const uint4*>(q + ch * 8));
-                    raw[n][u][0] = r.x;
-                    raw[n][u][1] = r.y;
-                    raw[n][u][2] = r.z;
-                    raw[n][u][3] = r.w;
+                    raw[u][0] = r.x;
+                    raw[u][1] = r.y;
+                    raw[u][2] = r.z;
+                    raw[u][3] = r.w;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) raw[n][u][i >> 1] |= (uint32_t)q[ch * 8 + i] << (16 * (i & 1));
+                    for (int i = 0; i < 8; ++i) raw[u][i >> 1] |= (uint32_t)q[ch * 8 + i] << (16 * (i & 1));
                 }
             }
         }
-    }
-#pragma unroll
+    };
+    fetch(0);
+#pragma unroll 1
     for (int n = 0; n < NT; ++n) {
         const int c = 8 * n + warp;
         float v[3][8];
@@ -315,10 +322,11 @@ __device__ __forceinline__ void load_query(const Mla4Args& a, int row, int block
         for (int u = 0; u < 3; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t b = raw[n][u][i >> 1] >> (16 * (i & 1)) & 0xffffu;
+                const uint32_t b = raw[u][i >> 1] >> (16 * (i & 1)) & 0xffffu;
                 v[u][i] = kBf16 ? __uint_as_float(b << 16) : __half2float(__ushort_as_half((uint16_t)b));
                 top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
             }
+        fetch(n + 1);
         top = __reduce_max_sync(0xffffffffu, top);
         const bool bad = top >= 0x7f800000u;
         // 2^k with top * 2^k in [2^14, 2^15); a head of zeros or of values below 2^-103 stays small
@@ -442,14 +450,11 @@ __device__ __forceinline__ bool score_unit(const Mla4Args& a, unsigned char* sm,
                 for (int r = 0; r < 4; ++r) S[i][n][r] = fmaf(s[2 * i + (r >> 1)], D[i][n][r], S[i][n][r]);
     };
 #pragma unroll 1
-    for (int gr = 0; gr < groups - 1; ++gr) {
+    for (int gr = 0; gr < groups; ++gr) {
         products(2 * gr, true);
-        products(2 * gr + 1, false);
+        if (2 * gr + 1 < blocks) products(2 * gr + 1, false);
         scaled(gr);
     }
-    products(2 * (groups - 1), true);
-    if (a.sh.rope > 64) products(2 * groups - 1, false);
-    scaled(groups - 1);
 
     // scores, and the lane's largest of each head
     const float* factor = reinterpret_cast<const float*>(query + (a.sh.kv_lora + a.sh.rope) / 32 * NT * 512);
@@ -620,7 +625,7 @@ __device__ __forceinline__ void follow(Sum<NT>& s, int group, int lane, const fl
 template <int NT>
 __device__ __forceinline__ void sum_tile(const Mla4Args& a, Sum<NT>& s, int group, int lane, const unsigned char* rows,
                                          const unsigned char* probs, const unsigned char* ratios, const float* stats) {
-    constexpr int kUnits = kTile / kUnit, kSteps = kTile / 16;
+    static_assert(kUnit == 32);
     const int g = lane >> 2, t = lane & 3, rb = a.sh.row_bytes();
     const unsigned char* p = rows + t * rb + 4 * g;
     struct Step {
@@ -637,31 +642,32 @@ __device__ __forceinline__ void sum_tile(const Mla4Args& a, Sum<NT>& s, int grou
             f.q[n] = *reinterpret_cast<const uint2*>(probs + unit * Smem<NT>::kProbBytes + (n * 8 + g) * 64 + 8 * swizzled(4 * half + t, g));
     };
     fetch(0, at[0]);
+#pragma unroll 1
+    for (int unit = 0; unit < kTile / kUnit; ++unit) {
+        const float* u = stats + unit * Smem<NT>::kStats;
+        follow<NT>(s, group, lane, u);
+        if (lane < 8 * NT) s.L += u[8 * NT + lane];
 #pragma unroll
-    for (int st = 0; st < kSteps; ++st) {
-        if (st % (kSteps / kUnits) == 0) {
-            const float* u = stats + st / (kSteps / kUnits) * Smem<NT>::kStats;
-            follow<NT>(s, group, lane, u);
-            if (lane < 8 * NT) s.L += u[8 * NT + lane];
-        }
-        const Step& f = at[st & 1];
-        if (st + 1 < kSteps) fetch(st + 1, at[(st + 1) & 1]);
-        uint32_t B[NT][2];
+        for (int st = 0; st < kUnit / 16; ++st) {
+            const Step& f = at[st];
+            if (st == 0 || unit + 1 < kTile / kUnit) fetch(2 * unit + st + 1, at[st ^ 1]);
+            uint32_t B[NT][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][0]) : "r"(f.q[n].x), "r"(f.r.x));
-            asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][1]) : "r"(f.q[n].y), "r"(f.r.y));
-        }
+            for (int n = 0; n < NT; ++n) {
+                asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][0]) : "r"(f.q[n].x), "r"(f.r.x));
+                asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(B[n][1]) : "r"(f.q[n].y), "r"(f.r.y));
+            }
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {  // nibbles 4 part .. 4 part + 3 of two positions side by side
-            uint32_t x[4], y[4];
-            unpack8(__byte_perm(f.w[0], f.w[1], part ? 0x7632 : 0x5410), x);
-            unpack8(__byte_perm(f.w[2], f.w[3], part ? 0x7632 : 0x5410), y);
+            for (int part = 0; part < 2; ++part) {  // nibbles 4 part .. 4 part + 3 of two positions side by side
+                uint32_t x[4], y[4];
+                unpack8(__byte_perm(f.w[0], f.w[1], part ? 0x7632 : 0x5410), x);
+                unpack8(__byte_perm(f.w[2], f.w[3], part ? 0x7632 : 0x5410), y);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {  // product 2 part + c: nibbles 4 part + 2 c and + 1
-                const uint32_t A[4] = {x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1]};
+                for (int c = 0; c < 2; ++c) {  // product 2 part + c: nibbles 4 part + 2 c and + 1
+                    const uint32_t A[4] = {x[2 * c], x[2 * c + 1], y[2 * c], y[2 * c + 1]};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(s.O[2 * part + c][n], A, B[n][0], B[n][1], s.O[2 * part + c][n]);
+                    for (int n = 0; n < NT; ++n) mma_f16(s.O[2 * part + c][n], A, B[n][0], B[n][1], s.O[2 * part + c][n]);
+                }
             }
         }
     }
@@ -701,14 +707,14 @@ __device__ __forceinline__ void finish_item(const Mla4Args& a, const Sum<NT>& s,
     const int slot = 2 * blockIdx.x + (w.first == 0 ? 1 : 0), lat = part * 64 + 8 * g;
     float2* stat = reinterpret_cast<float2*>(a.ws + ws.stats) + (size_t)slot * a.block_heads;
     float* sums = reinterpret_cast<float*>(a.ws + ws.sums) + (size_t)slot * a.block_heads * a.sh.kv_lora;
+    const float inv = whole && s.L != 0.f ? 1.f / s.L : 1.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int c = column_head(n, 2 * t + e);
-            const float L = __shfl_sync(0xffffffffu, s.L, 8 * n + 2 * t + e), R = __shfl_sync(0xffffffffu, s.R, 8 * n + 2 * t + e);
+            const float unit = s.ref * __shfl_sync(0xffffffffu, inv, 8 * n + 2 * t + e);
             if (c >= a.block_heads || h0 + c >= a.n_heads) continue;
-            const float unit = s.ref * (whole && L != 0.f ? 1.f / L : 1.f);
             float v[8];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -722,13 +728,14 @@ __device__ __forceinline__ void finish_item(const Mla4Args& a, const Sum<NT>& s,
                 d[0] = make_float4(v[0], v[1], v[2], v[3]);
                 d[1] = make_float4(v[4], v[5], v[6], v[7]);
             }
-            if (part == 0 && g == 0) {
-                if (!whole)
-                    stat[c] = make_float2(R, L);
-                else if (a.lse)
-                    a.lse[(size_t)w.row * a.n_heads + h0 + c] = R == -INFINITY && L == 0.f ? -INFINITY : R + logf(L);
-            }
         }
+    const int c = column_head(lane >> 3, lane & 7);
+    if (part == 0 && lane < 8 * NT && c < a.block_heads && h0 + c < a.n_heads) {
+        if (!whole)
+            stat[c] = make_float2(s.R, s.L);
+        else if (a.lse)
+            a.lse[(size_t)w.row * a.n_heads + h0 + c] = s.R == -INFINITY && s.L == 0.f ? -INFINITY : s.R + logf(s.L);
+    }
 }
 
 // -------------------------------------------------------------- kernel
@@ -745,11 +752,14 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
     const Smem<NT> L(a.sh, a.stages);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
+#pragma unroll 1
         for (int i = 0; i < a.stages; ++i) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], kSumWarps);
         }
+#pragma unroll 1
         for (int i = 0; i < kPairs; ++i) mbar_init(&prob_full[i], kTile / kUnit);
+#pragma unroll 1
         for (int i = 0; i < kScoreWarps; ++i) mbar_init(&chain[i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&query_full[i], kScoreWarps);
@@ -765,6 +775,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
     const int per = (a.n_rows + kAtThreads - 1) / kAtThreads;
     const int r0 = min(a.n_rows, tid * per), r1 = min(a.n_rows, r0 + per);
     long long mine = 0;
+#pragma unroll 1
     for (int r = r0; r < r1; ++r) mine += tiles_of(row_length(a, r));
     long long run = mine;
 #pragma unroll
@@ -775,6 +786,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
     if (lane == 31) scan[warp] = run;
     __syncthreads();
     long long before = run - mine, rows_total = 0;
+#pragma unroll 1
     for (int w = 0; w < kAtThreads / 32; ++w) {
         if (w < warp) before += scan[w];
         rows_total += scan[w];
@@ -797,6 +809,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
     const long long lo = part_lo, hi = part_hi;
     if (hi > lo) {
         long long at = before * a.blocks;
+#pragma unroll 1
         for (int r = r0; r < r1; ++r) {
             const long long n = tiles_of(row_length(a, r)), end = at + n * a.blocks;
             if (lo >= at && lo < end) {
@@ -806,6 +819,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
             // items that begin in this part: whether they go on past it
             if (by_item) {
                 long long first = at;
+#pragma unroll 1
                 for (int b = 0; b < a.blocks; ++b, first += n)
                     if (first >= lo && first < hi)
                         joins[r * a.blocks + b] = Join{r * a.blocks + b, first + n > hi ? (int)blockIdx.x : -1,
@@ -833,6 +847,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
         const size_t pb = a.sh.page_bytes();
         int i = 0;
         Place at;
+#pragma unroll 1
         while (ok && w.next()) {
             const int req = a.row_req[w.row];
             const int32_t* ids = a.table + (size_t)(w.len > 0 ? req : 0) * a.table_stride;
@@ -841,6 +856,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
             int base = w.first * spans / tiles_per_page;
             int now = base + lane < n_ids ? ids[base + lane] : -1;
             int next = base + 32 + lane < n_ids ? ids[base + 32 + lane] : -1;
+#pragma unroll 1
             for (int tile = w.first; tile < w.end; ++tile, ++i, at.forward(1, stages)) {
                 const int stage = at.stage;
                 if (i >= stages && !warp_wait(&empty[stage], at.phase ^ 1u)) {
@@ -858,6 +874,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
                 const bool held = lane < spans && id >= 0 && id < a.n_pages;
                 const unsigned there = __ballot_sync(0xffffffffu, held);
                 uint64_t bits = 0;
+#pragma unroll 1
                 for (int s = 0; s < spans; ++s)
                     if (there >> s & 1) bits |= (per_page == 64 ? ~0ull : (1ull << per_page) - 1) << (s * per_page);
                 const long long rest = w.len - (long long)tile * kTile;
@@ -888,7 +905,8 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
             }
         }
         if (!ok)  // let the copies in flight land before leaving
-            for (int j = max(0, i - stages); j < i; ++j) mbar_wait_bounded(&full[j % stages], (j / stages) & 1);
+#pragma unroll 1
+            for (int j = max(0, i - stages); j < i; ++j) warp_wait(&full[j % stages], (j / stages) & 1);
     } else if (warp < kScoreWarps) {
         grow_registers<kScoreRegs>();
         const int per = a.sh.page < kTile ? a.sh.page : kTile, per_log = 31 - __clz(per);  // positions of a page in a tile
@@ -902,19 +920,18 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
         // Two queries' room: a warp loads its share of the next item's once it
         // has done a unit of this one, when the others are through with the
         // item before. Nobody waits for all at an item's end.
-        bool more = w.next();
-        if (more) {
-            load_query<NT, kBf16>(a, w.row, w.block, sm + L.qf, warp, lane);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&query_full[0]);
-        }
-        for (unsigned item = 0; more && ok; ++item) {
-            unsigned char* query = sm + L.qf + (item & 1) * L.query;
-            const unsigned u0 = u;
-            u += (unsigned)(w.end - w.first) * kUnits;
-            ok = warp_wait(&query_full[item & 1], item >> 1 & 1);
+        // Pass k has the units of item k - 1 and loads item k's query.
+#pragma unroll 1
+        for (unsigned pass = 0;; ++pass) {
+            const unsigned u0 = u, now = pass + 1 & 1;
+            const unsigned char* query = sm + L.qf + now * L.query;
+            if (pass > 0) {
+                u += (unsigned)(w.end - w.first) * kUnits;
+                ok = warp_wait(&query_full[now], pass - 1 >> 1 & 1);
+            }
             bool loaded = false;
-            more = w.next();  // from here on w is the next item
+            const bool more = w.next();  // from here on w is the next item
+#pragma unroll 1
             for (; ok; mine += kScoreWarps, at.forward(kScoreWarps / kUnits, stages)) {
                 const bool unit = mine < u;
                 if (unit) {
@@ -936,17 +953,17 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
                 }
                 if (!loaded && more) {
                     loaded = true;
-                    const unsigned to = item + 1;
-                    if (to >= 2) ok = warp_wait(&query_empty[to & 1], (to >> 1 & 1) ^ 1);
+                    if (pass >= 2) ok = warp_wait(&query_empty[pass & 1], (pass >> 1 & 1) ^ 1);
                     if (!ok) break;
-                    load_query<NT, kBf16>(a, w.row, w.block, sm + L.qf + (to & 1) * L.query, warp, lane);
+                    load_query<NT, kBf16>(a, w.row, w.block, sm + L.qf + (pass & 1) * L.query, warp, lane);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&query_full[to & 1]);
+                    if (lane == 0) mbar_arrive(&query_full[pass & 1]);
                 }
                 if (!unit) break;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&query_empty[item & 1]);
+            if (pass > 0 && lane == 0) mbar_arrive(&query_empty[now]);
+            if (!more || !ok) break;
         }
     } else {
         grow_registers<kSumRegs>();
@@ -955,6 +972,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
         const int rb = a.sh.row_bytes();
         unsigned u = 0;
         Place at;
+#pragma unroll 1
         while (ok && w.next()) {
             Sum<NT> s;
             s.ref = s.L = 0.f;
@@ -965,6 +983,7 @@ __global__ void __launch_bounds__(kAtThreads, 1) mla4_attention_kernel(Mla4Args 
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) s.O[b][n][r] = 0.f;
+#pragma unroll 1
             for (int tile = w.first; tile < w.end; ++tile, at.forward(1, stages), ++u) {
                 // the tile's codes are there too: its scores were formed from them
                 const unsigned pair = u % kPairs;
@@ -1002,6 +1021,7 @@ __global__ void __launch_bounds__(kJoinGroup* kJoinGroups) mla4_join_kernel(Mla4
         // a wait gave up: no result is to be taken for one
         const long long n = (long long)a.n_rows * a.n_heads * a.sh.kv_lora;
         const long long all = (long long)gridDim.x * gridDim.y * blockDim.x;
+#pragma unroll 1
         for (long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + tid; i < n; i += all) {
             const long long rh = i / a.sh.kv_lora;
             const long long at = rh / a.n_heads * a.out_row + rh % a.n_heads * a.out_head + i % a.sh.kv_lora;
@@ -1024,10 +1044,12 @@ __global__ void __launch_bounds__(kJoinGroup* kJoinGroups) mla4_join_kernel(Mla4
         if (c < heads) {
             const float2* stats = reinterpret_cast<const float2*>(a.ws + ws.stats) + c;
             const float* sums = reinterpret_cast<const float*>(a.ws + ws.sums) + (size_t)c * a.sh.kv_lora + 4 * at;
+#pragma unroll 1
             for (int k = lane; k < parts; k += 32) M = fmaxf(M, stats[slot(k)].x);  // every warp for itself
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
             const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 1
             for (int k = lane; k < parts; k += 32) {
                 const float2 st = stats[slot(k)];
                 l += exp_of(st.x - base) * st.y;
@@ -1035,7 +1057,7 @@ __global__ void __launch_bounds__(kJoinGroup* kJoinGroups) mla4_join_kernel(Mla4
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
             if (latents) {
-#pragma unroll 8
+#pragma unroll 4
                 for (int k = group / at_once; k < parts; k += sharing) {
                     const float4 v = *reinterpret_cast<const float4*>(sums + slot(k) * a.sh.kv_lora);
                     const float wk = exp_of(stats[slot(k)].x - base);
@@ -1050,6 +1072,7 @@ __global__ void __launch_bounds__(kJoinGroup* kJoinGroups) mla4_join_kernel(Mla4
             part_sum[group][at] = o;
             __syncthreads();
             if (group < at_once)
+#pragma unroll 1
                 for (int i = group + at_once; i < kJoinGroups; i += at_once) {
                     const float4 v = part_sum[i][at];
                     o.x += v.x;
