@@ -10,14 +10,14 @@
 // would; a group whose scale rounds to zero holds zeros.
 //
 // Both should be bound by memory traffic, which the store is only with few
-// instructions a value: no conversion to integers, no integer division, ties
+// instructions a value (14): no conversion to integers, no integer division, ties
 // decided by one corrected quotient for all, magnitudes of 16-bit values two at
 // a time. Four lanes share a group, so that what is done once for a group costs
 // little, and a block has 16 rows: 16-byte loads (stores) of four lanes touch
 // 64 bytes in a row, two shuffles give a group's largest magnitude, and no load
 // waits for another.
 //
-// Measured: 60001 rows of 512 + 64 bf16 (87 MB) take 18.5 us, 4.7 TB/s; with
+// Measured: 60001 rows of 512 + 64 bf16 (87 MB) take 18.8 us, 4.6 TB/s; with
 // eight lanes to a group and the same arithmetic one at a time 27 us. 20000 rows
 // of 256 + 64 to fp32 (30 MB) take 6.7 us, a launch included.
 #include <cstdint>
@@ -38,6 +38,7 @@ constexpr int kBlockRows = 16;
 constexpr int kGroupLanes = 4;  // a block has kBlockRows * groups * kGroupLanes threads: 128 to 320
 constexpr int kMostThreads = kBlockRows * kKv4MaxGroups * kGroupLanes;
 constexpr float kWhole = 12582912.f;  // 1.5 * 2^23: x + kWhole is x rounded to an integer, half to even, in its low bits
+constexpr float kSmallScale = 1e-35f;         // from here on the last bit of a remainder (quotients of 1/2 and more) is at 2^-148 or above
 constexpr unsigned kWholeBits = 0x4b400000u;  // of kWhole
 
 struct RowArgs {
@@ -108,10 +109,10 @@ __device__ __forceinline__ void put(T* p, const float (&v)[kN]) {
     }
 }
 
-// rint(x / s) of two values, as numbers kWhole + rint, for |x / s| < 8, 2^-126
-// <= s and inv = 1 / s rounded: the quotient's first estimate is within two
-// units of its last place, so the remainder r is exact, and its correction is
-// off by less than 2^-45 of the quotient. That cannot change what q rounds to:
+// rint(x / s) of two values, as numbers kWhole + rint, for |x / s| < 8, s >=
+// kSmallScale and inv = 1 / s rounded: the quotient's first estimate is within
+// two units of its last place, so the remainder r is exact, and its correction
+// is off by less than 2^-45 of the quotient. That cannot change what q rounds to:
 // x / s with an 8-bit s lies at least 2^-34 of itself from every midpoint of
 // two fp32 numbers, or x would have more than 24 bits.
 __device__ __forceinline__ void whole_of(float x0, float x1, Two minus_s, Two inv, unsigned& w0, unsigned& w1) {
@@ -122,7 +123,8 @@ __device__ __forceinline__ void whole_of(float x0, float x1, Two minus_s, Two in
     w1 = __float_as_uint(f1);
 }
 
-// The same by the division, for scales below the normal numbers.
+// The same by the division, for smaller scales: r would fall below the last
+// place of the smallest numbers, 1 / s overflow, a quotient pass 8.
 __device__ __noinline__ unsigned code_of_small(float x, float s) {
     return (unsigned)(min(max((int)rintf(__fdiv_rn(x, s)), -7), 7) + 8);
 }
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(kMostThreads) kv4_store_kernel(RowArgs a) {
     const __nv_bfloat16 sb = bad ? __ushort_as_bfloat16(0x7fc0) : __float2bfloat16_rn(__fdiv_rn(top, 7.f));
     const float s = __bfloat162float(sb);
     const bool zero = bad || s == 0.f;
-    const bool small = s < 1e-37f;  // its reciprocal could overflow, its quotients be beyond 8
+    const bool small = s < kSmallScale;
     const float inv = __frcp_rn(s);
     const Two minus_s(-s, -s), inv2(inv, inv);
 #pragma unroll

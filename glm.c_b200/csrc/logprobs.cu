@@ -27,9 +27,9 @@
 // than the GPU holds CTAs; the CTAs of a cluster meet in distributed shared
 // memory. No workspace, no second launch.
 //
-// Measured: 64 rows of 154880 fp32 with the best 20: 15.0 us, of which a launch
+// Measured: 64 rows of 154880 fp32 with the best 20: 15.1 us, of which a launch
 // by itself is about 8 and the reading 6; 1500 rows of 32003 bf16, no best:
-// 22.9 us, 4.2 TB/s, where the exponentials take half of their unit's time and
+// 22.8 us, 4.2 TB/s, where the exponentials take half of their unit's time and
 // the starts and ends of 1500 CTAs the rest.
 #include <cfloat>
 #include <cmath>
@@ -50,8 +50,8 @@ namespace {
 
 // Threads of a CTA, CTAs that an SM is to hold, 16-byte loads of a thread in
 // flight. The best tokens cost every CTA sorts and merges: fewer, larger CTAs
-// (64 rows of 154880 fp32: 15.0 us, at 256 threads 16.7). Without them more
-// and smaller ones hide the loads (1500 rows of 32003 bf16: 22.9 us, with 4
+// (64 rows of 154880 fp32: 15.1 us, at 256 threads 16.7). Without them more
+// and smaller ones hide the loads (1500 rows of 32003 bf16: 22.8 us, with 4
 // CTAs and 4 loads 24.6, at 512 threads 31).
 template <bool kTop>
 struct LpShape {

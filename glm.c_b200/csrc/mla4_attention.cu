@@ -48,19 +48,24 @@
 // barrier for both.
 //
 // What bounds it, measured at 16 requests of 32768 positions, 20 heads of 512 +
-// 64 (153 MB of cache): 128 us, 1.19 TB/s. The products take 43 % of the tensor
-// pipe's time, the instructions around them (unpacking, scales, waits) keep 53 %
-// of the issue slots; 16 such warps are all that an SM holds, too
-// few to fill the rest. At one request of 1500 positions it takes 21 us, most
-// of it three dependent steps: the query's load, one tile a CTA, the join.
-// Tried on the way here and slower at that size: 12 score and 4 sum warps (200
-// us: spills), the sum warps in units of 32 positions (137 us: a wait for each),
-// the codes as f16 numbers below 2^-14, unbiased by -8 times the query's sum
-// (137 us, and four times the error in scores of hundreds),
-// tcgen05 with the codes spread to bytes in shared memory (192 us: the warps
-// that spread the codes and read the accumulators back are the bound).
-// m16n8k32 e4m3, for which the codes need no arithmetic, issues at 0.21 a clock
-// of an SM against 0.50 for f16: no faster.
+// 64 (153 MB of cache): 121 us, 1.27 TB/s. The products alone would keep the
+// tensor pipe busy for 48 us of it, the instructions around them (unpacking,
+// scales, waits) the issue slots for about 65; 16 such warps are all that an SM
+// holds, too few to cover each other's chains of loads, unpacking and products.
+// At one request of 1500 positions it takes 18 us, most of it two launches and
+// the dependent steps between them: lengths, table, one tile a CTA, the join.
+// Code size counts at both ends: with every loop unrolled and a copy of the
+// query's loading for the first item (140 KB against 83) the same took 128 and
+// 20.5 us.
+// Tried on the way here and slower at the large size: 12 score and 4 sum warps
+// (200 us: spills), the sum warps in units of 32 positions (137 us: a wait for
+// each), the codes as f16 numbers below 2^-14, unbiased by -8 times the query's
+// sum (137 us, and four times the error in scores of hundreds), 17 warps
+// without a split of the registers (161 us: five of them share a quarter of the
+// SM, which leaves 96 each), tcgen05 with the codes spread to bytes in shared
+// memory (192 us: the warps that spread the codes and read the accumulators
+// back are the bound). m16n8k32 e4m3, for which the codes need no arithmetic,
+// issues at 0.21 a clock of an SM against 0.50 for f16.
 
 #include <cfloat>
 #include <climits>
