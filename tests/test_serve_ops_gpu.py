@@ -221,6 +221,27 @@ def test_rows_special_values(lib):
     np.testing.assert_array_equal(v.cpu().numpy(), np.concatenate([rv.reshape(12, kv), pv[:, 0]], 1))
 
 
+@pytest.mark.parametrize("low,high", [(-149, -110), (-122, -100), (-100, 0), (0, 124)])
+def test_rows_quotients_beside_the_halves(lib, low, high):
+    """Values a few units of their last place around (k + 1/2) s, for scales of every magnitude: codes are equal to
+    rint of the rounded quotient bit for bit, in the fast arithmetic and below it."""
+    kv, rope, page, n = 512, 64, 64, 256
+    rng = np.random.default_rng(low + 200)
+    scale = np.ldexp(rng.integers(128, 256, (n, kv // GROUP, 1)) / 128.0, rng.integers(low, high, (n, kv // GROUP, 1)))
+    half = rng.integers(-7, 7, (n, kv // GROUP, GROUP)) + 0.5
+    x = (half * scale).astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-3, 4, x.shape) * (np.abs(x) > 1e-44)).astype(np.int32).view(np.float32)
+    x[..., 17] = (7 * scale[..., 0]).astype(np.float32)  # the largest: the scale is the one drawn
+    x = np.ascontiguousarray(x.reshape(n, kv))
+    pages, cache = pool_of(lib, n // page, kv, rope, page)
+    slots = torch.arange(n, device="cuda")
+    lib.kv4_store_async(cache, torch.from_numpy(x).cuda(), torch.from_numpy(np.ascontiguousarray(x[:, :rope])).cuda(), slots)
+    v, s = pool_rows(pages, slots, kv, rope, page)
+    rv, rs = quantise(x.reshape(n, -1, GROUP))
+    np.testing.assert_array_equal(s[:, :-1].cpu().numpy(), rs)
+    np.testing.assert_array_equal(v[:, :kv].cpu().numpy(), rv.reshape(n, kv))
+
+
 def test_rows_outside_the_pool_are_left_out(lib):
     kv, rope, page, n_pages = 128, 64, 16, 3
     pages, cache = pool_of(lib, n_pages, kv, rope, page, fill=0x11)
